@@ -12,7 +12,9 @@ from .diffsinger import ENCODERS, DiffSinger, NaiveProjectionEncoder, pitch_to_s
 from .refinegan import RefineGAN, RefineGANGenerator  # noqa: F401
 from .hifisinger import HiFiSinger  # noqa: F401
 from .inference import SVCModel, inference_model, load_checkpoint  # noqa: F401
+from .ops import attention, attention_backward, attention_forward  # noqa: F401
 from . import segments  # noqa: F401
 
 __all__ = ["DENOISERS", "DIFFUSIONS", "VOCODERS", "install", "WaveNet", "ConvNext", "TransformerDecoderDenoiser", "GaussianDiffusion", "NsfHifiGAN", "Generator",
-           "PitchAdjustableMelSpectrogram", "ENCODERS", "DiffSinger", "NaiveProjectionEncoder", "pitch_to_scale", "repeat_expand", "RefineGAN", "RefineGANGenerator", "HiFiSinger", "SVCModel", "load_checkpoint", "inference_model"]
+           "PitchAdjustableMelSpectrogram", "ENCODERS", "DiffSinger", "NaiveProjectionEncoder", "pitch_to_scale", "repeat_expand", "RefineGAN", "RefineGANGenerator", "HiFiSinger", "SVCModel", "load_checkpoint", "inference_model",
+           "attention", "attention_forward", "attention_backward"]

@@ -67,6 +67,16 @@ class MelDesc(C.Structure):
                 ("n_mels", C.c_int), ("f_min", C.c_float), ("f_max", C.c_float)]
 
 
+class Bht(C.Structure):
+    _fields_ = [("data", C.c_void_p), ("b", C.c_longlong), ("h", C.c_longlong), ("t", C.c_longlong)]
+
+
+class AttnDesc(C.Structure):
+    _fields_ = [(n, C.c_int) for n in ("dtype", "batch", "heads", "kv_heads", "q_len", "k_len", "head_dim", "causal")] + [("scale", C.c_float)]
+
+
+DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+
 _P = C.c_void_p
 _SIGS = {
     "fdx_version": (C.c_int, []),
@@ -114,6 +124,10 @@ _SIGS = {
     "fdx_mel_filterbank": (C.c_int, [C.POINTER(MelDesc), _P]),
     "fdx_mel_forward": (C.c_int, [_P, _P, C.c_int, C.c_int, C.c_float, C.c_float, C.c_int, _P, _P]),
     "fdx_mel_stats": (C.c_int, [_P, C.POINTER(C.c_long), C.POINTER(C.c_long), C.POINTER(C.c_int)]),
+    "fdx_attn_forward_workspace": (C.c_int, [C.POINTER(AttnDesc), C.POINTER(C.c_size_t)]),
+    "fdx_attn_forward": (C.c_int, [_P, C.POINTER(AttnDesc), C.POINTER(Bht), C.POINTER(Bht), C.POINTER(Bht), _P, C.POINTER(Bht), _P, _P, C.c_size_t, _P]),
+    "fdx_attn_backward_workspace": (C.c_int, [C.POINTER(AttnDesc), C.POINTER(C.c_size_t)]),
+    "fdx_attn_backward": (C.c_int, [_P, C.POINTER(AttnDesc)] + [C.POINTER(Bht)] * 5 + [_P, _P] + [C.POINTER(Bht)] * 3 + [_P, C.c_size_t, _P]),
     "fdx_bcast_arena": (C.c_int, [_P, C.c_size_t, _P, C.c_int, _P]),
     "fdx_refinegan_num_weights": (C.c_int, [C.POINTER(RefineGanDesc)]),
     "fdx_refinegan_num_noises": (C.c_int, [C.POINTER(RefineGanDesc)]),

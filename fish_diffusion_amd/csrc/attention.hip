@@ -1,0 +1,777 @@
+// attention.hip -- attention with its backward pass, as callable operators (fdx_attn_*).
+//
+//   s_ij = scale q_i.k_j (-inf where key j is masked, or causal and j > i + Tk - Tq)    P = exp(s - lse)    o = P v
+//   delta_i = do_i.o_i    dS = P (do v^T - delta)    dq = scale dS k    dk = scale dS^T q    dv = P^T do
+//
+// The G query heads that share a key / value head are one list of R = G * Tq rows: a tile of rows may cross heads, K / V are staged once for
+// all of them, and the sum of dk / dv over the shared heads is the ordinary sum over rows (no atomics: the same bits on every run).
+//
+// Every kernel holds its 32 rows (keys, for dk / dv) per wave as the COLUMN operand, so that a lane owns one row of the softmax (half of it:
+// lanes l and l + 32 hold 16 of 32 keys each).  Forward and dq compute S^T = K Q^T and then O^T += V^T P^T, dQ^T += K^T dS^T: the accumulator
+// of the first product is the operand of the second one without leaving its lane (tileops.hip.h), statistics need one exchange with the other half.
+// dk / dv mirror it with S = Q K^T and dK^T += Q^T dS, dV^T += dO^T P.  Scores and statistics are fp32; P and dS are rounded once to the
+// operand type (fp32: not at all) to enter the matrix instruction, as the inputs were.
+// dq and dk / dv are two passes that each recompute S and P (7 products instead of 5): sharing one would need atomics on dq or 1/64 of the
+// score matrix' traffic in partial sums, 4 bytes per (query, key) at head size 64 against 256 flops.
+#include "tileops.hip.h"
+
+#include <algorithm>
+#include <climits>
+#include <cmath>
+
+using namespace fdx;
+
+namespace {
+
+struct Str { long b, h, t; };
+struct AttnArgs {
+  const void *q, *k, *v, *go;
+  void *o, *dq, *dk, *dv;
+  Str sq, sk, sv, sgo, so, sdq, sdk, sdv;
+  const uint8_t* mask;   // [B][Tk], 1 = masked
+  float *lse, *delta, *part;
+  int B, H, Hkv, G, Tq, Tk, D, R, off, causal, splits, tiles;
+  float c, scale;        // c = scale * log2(e)
+};
+
+constexpr float kLn2 = 0.69314718055994530942f, kLog2e = 1.44269504088896340736f;
+__device__ inline float inf() { return __builtin_inff(); }
+__device__ inline float exp2_(float x) { return __builtin_amdgcn_exp2f(x); }
+__device__ inline float other_half(float x) { return __shfl_xor(x, 32, 64); }
+
+// workgroup -> (batch and kv head, tile, split).  Workgroups go to the 8 XCDs in turn: where the heads divide, all tiles of a head run on one
+// XCD and find its K / V in that XCD's L2.  Late (causal: long) tiles start first.
+__device__ inline void decode(const AttnArgs& a, int& bh, int& tile, int& split) {
+  const int nb = a.B * a.Hkv, per = a.tiles * a.splits, i = blockIdx.x;
+  int j;
+  if (nb % 8 == 0) { bh = (i & 7) + 8 * ((i >> 3) / per); j = (i >> 3) % per; }
+  else { bh = i / per; j = i % per; }
+  split = j % a.splits;
+  tile = a.tiles - 1 - j / a.splits;
+}
+
+// one past the last key any row of [r0, r1] sees
+__device__ inline int key_end(const AttnArgs& a, int r0, int r1) {
+  if (!a.causal) return a.Tk;
+  const int t = r0 / a.Tq == r1 / a.Tq ? r1 % a.Tq : a.Tq - 1;
+  return max(0, min(a.Tk, t + a.off + 1));
+}
+
+// TK rows of DH elements on their way from memory to LDS, in registers of the 256 threads
+template <typename T, int DH, int TK> struct Stage {
+  typedef Tile<T, DH> Tl;
+  static constexpr int NV = TK * Tl::CPR / 256;
+  static_assert(NV * 256 == TK * Tl::CPR, "whole vectors per thread");
+  uint4 r[NV];
+  static __device__ inline int row(int i) { return ((int)threadIdx.x + 256 * i) / Tl::CPR; }
+  static __device__ inline int chunk(int i) { return ((int)threadIdx.x + 256 * i) % Tl::CPR; }
+  template <typename F> __device__ inline void load(F&& src, int D) {   // src(row, i): row's address or null (zeros)
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const T* p = src(row(i), i);
+      r[i] = p && chunk(i) * Elem<T>::VEC < D ? *reinterpret_cast<const uint4*>(p + chunk(i) * Elem<T>::VEC) : uint4{0, 0, 0, 0};
+    }
+  }
+  __device__ inline void store(uint4* lds) const {
+#pragma unroll
+    for (int i = 0; i < NV; ++i) lds[Tl::at(row(i), chunk(i))] = r[i];
+  }
+};
+
+// a wave's 32 rows of DH elements as column operands (lane: row lane & 31), zeros beyond D and where p is null
+template <typename T, int DH> __device__ inline void load_rows(typename Elem<T>::frag* f, const T* p, int D, int lane) {
+#pragma unroll
+  for (int s = 0; s < DH / Elem<T>::KS; ++s) {
+    const int e = (2 * s + (lane >> 5)) * Elem<T>::VEC;
+    f[s] = __builtin_bit_cast(typename Elem<T>::frag, p && e < D ? *reinterpret_cast<const uint4*>(p + e) : uint4{0, 0, 0, 0});
+  }
+}
+
+template <typename T> __device__ inline void store4(T* p, float a, float b, float c, float d) {
+  typedef T v4 __attribute__((ext_vector_type(4)));
+  *reinterpret_cast<v4*>(p) = v4{(T)a, (T)b, (T)c, (T)d};
+}
+
+// transposed accumulators acc[m] (row d, column = this lane's row) times f to a row of D elements
+template <typename T, int MT> __device__ inline void store_cols(T* p, const f32x16* acc, float f, int D, int lane) {
+#pragma unroll
+  for (int m = 0; m < MT; ++m)
+#pragma unroll
+    for (int b = 0; b < 4; ++b) {
+      const int d = 32 * m + 8 * b + 4 * (lane >> 5);
+      if (d < D) store4<T>(p + d, acc[m][4 * b] * f, acc[m][4 * b + 1] * f, acc[m][4 * b + 2] * f, acc[m][4 * b + 3] * f);
+    }
+}
+
+// the same to LDS as [32][DH] fp32 (chunks of 4 swizzled by the row), one such block per wave, and one element of the blocks' sum
+__device__ inline int red_at(int row, int d, int DH) { return row * DH + (((d >> 2) ^ (row & 7)) << 2); }
+template <int DH> __device__ inline void put_rows(float* red, const f32x16* acc, float f, int lane) {
+#pragma unroll
+  for (int m = 0; m < DH / 32; ++m)
+#pragma unroll
+    for (int q = 0; q < 4; ++q)
+      *reinterpret_cast<f32x4*>(red + red_at(lane & 31, 32 * m + 8 * q + 4 * (lane >> 5), DH)) =
+          f32x4{acc[m][4 * q] * f, acc[m][4 * q + 1] * f, acc[m][4 * q + 2] * f, acc[m][4 * q + 3] * f};
+}
+template <int DH> __device__ inline f32x4 sum_rows(const float* red, int row, int d) {
+  f32x4 v = {0, 0, 0, 0};
+#pragma unroll
+  for (int w = 0; w < 4; ++w) v += *reinterpret_cast<const f32x4*>(red + w * 32 * DH + red_at(row, d, DH));
+  return v;
+}
+
+// fp16: probabilities are carried times 2^14 (so <= 2^14), which keeps those down to 2^-28 normal numbers; every sum has the same factor.
+template <typename T> struct PShift { static constexpr float log2 = 0.f, back = 1.f; };
+template <> struct PShift<f16_t> { static constexpr float log2 = 14.f, back = 0x1p-14f; };
+
+// ---------------------------------------------------------------------------------------------------------------- forward
+// WQ waves take 32 rows each, the other factor of the 4 waves (WK) shares those rows and takes KT keys each of every step; their
+// (max, sum, O) meet in LDS at the end.  Online softmax: running maximum m of the raw scores, P = exp2(c s - c m).
+template <typename T, int DH, int WQ, int KT>
+__global__ __launch_bounds__(256) void k_attn_fwd(AttnArgs a) {
+  typedef Tile<T, DH> Tl;
+  typedef typename Elem<T>::frag frag;
+  constexpr int KS = Elem<T>::KS, WK = 4 / WQ, TK = KT * WK, NS = DH / KS, MT = DH / 32, NU = KT / 32, NP = 32 / KS;
+  constexpr int kTile = TK * Tl::CPR, kMerge = WK > 1 ? WK * 32 * DH / 4 : 0;   // in 16-byte units
+  __shared__ uint4 smem[2 * kTile > kMerge ? 2 * kTile : kMerge];
+  __shared__ float ml[2][4][32];
+  uint4 *const lk = smem, *const lv = smem + kTile;
+  int bh, tile, split;
+  decode(a, bh, tile, split);
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wq = wave / WK, wk = wave % WK, hi = lane >> 5;
+  const int b = bh / a.Hkv, hk = bh % a.Hkv;
+  const int r0 = tile * 32 * WQ, r = r0 + wq * 32 + (lane & 31), rc = min(r, a.R - 1), g = rc / a.Tq, t = rc - g * a.Tq;
+  const int kmax = key_end(a, r0, min(r0 + 32 * WQ, a.R) - 1), steps = (kmax + TK - 1) / TK;
+  const int lim = a.causal ? t + a.off : INT_MAX;
+  const T* const K = static_cast<const T*>(a.k) + b * a.sk.b + hk * a.sk.h;
+  const T* const V = static_cast<const T*>(a.v) + b * a.sv.b + hk * a.sv.h;
+  const uint8_t* const mask = a.mask ? a.mask + (long)b * a.Tk : nullptr;
+  frag qf[NS];
+  load_rows<T, DH>(qf, static_cast<const T*>(a.q) + b * a.sq.b + (hk * a.G + g) * a.sq.h + t * a.sq.t, a.D, lane);
+  f32x16 acc[MT];
+#pragma unroll
+  for (int m = 0; m < MT; ++m) acc[m] = f32x16{0};
+  float mx = -inf(), l = 0.f;
+
+  Stage<T, DH, TK> sk, sv;
+  unsigned long long bits_next = 0;
+  auto fetch = [&](int st) {
+    const int k0 = st * TK;
+    const int kk = k0 + wk * KT + lane;
+    bits_next = __ballot(lane < KT && kk < a.Tk && !(mask && mask[min(kk, a.Tk - 1)]));
+    auto ok = [&](int row) { const int key = k0 + row; return key < a.Tk && !(mask && mask[key]); };   // masked rows enter as zeros: 0 * NaN never happens
+    sk.load([&](int row, int) { return ok(row) ? K + (long)(k0 + row) * a.sk.t : nullptr; }, a.D);
+    sv.load([&](int row, int) { return ok(row) ? V + (long)(k0 + row) * a.sv.t : nullptr; }, a.D);
+  };
+  if (split < steps) fetch(split);
+  for (int st = split; st < steps; st += a.splits) {
+    __syncthreads();
+    sk.store(lk);
+    sv.store(lv);
+    const unsigned long long bits = bits_next;
+    __syncthreads();
+    if (st + a.splits < steps) fetch(st + a.splits);
+    if (bits == 0) continue;   // (the wave's keys are all masked; the barriers are outside)
+    f32x16 s[NU];
+#pragma unroll
+    for (int u = 0; u < NU; ++u) {
+      s[u] = f32x16{0};
+#pragma unroll
+      for (int i = 0; i < NS; ++i) s[u] = Elem<T>::mma(Tl::row(lk, wk * KT + 32 * u + (lane & 31), 2 * i + hi), qf[i], s[u]);
+    }
+    const int rel = lim - (st * TK + wk * KT);   // last visible key of this lane's row, relative
+    const unsigned long long full = KT == 64 ? ~0ull : (1ull << KT) - 1;
+    if (!__all(bits == full && rel >= KT - 1)) {
+      unsigned long long ok = bits & (rel >= 63 ? ~0ull : rel < 0 ? 0ull : (2ull << rel) - 1);
+#pragma unroll
+      for (int u = 0; u < NU; ++u) {
+        const unsigned w = (unsigned)(ok >> (32 * u)) >> (4 * hi);
+#pragma unroll
+        for (int e = 0; e < 16; ++e) s[u][e] = (w >> (8 * (e >> 2) + (e & 3))) & 1 ? s[u][e] : -inf();
+      }
+    }
+    float mt = mx;
+#pragma unroll
+    for (int u = 0; u < NU; ++u)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) mt = fmaxf(mt, s[u][e]);
+    mt = fmaxf(mt, other_half(mt));
+    const float mc = mt == -inf() ? 0.f : mt * a.c;
+    const float alpha = exp2_(mx * a.c - mc);
+    mx = mt;
+    float sum = 0.f;
+#pragma unroll
+    for (int u = 0; u < NU; ++u)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) {
+        s[u][e] = exp2_(__builtin_fmaf(s[u][e], a.c, PShift<T>::log2 - mc));
+        sum += s[u][e];
+      }
+    l = l * alpha + sum;
+#pragma unroll
+    for (int m = 0; m < MT; ++m) acc[m] *= alpha;
+#pragma unroll
+    for (int u = 0; u < NU; ++u)
+#pragma unroll
+      for (int p = 0; p < NP; ++p) {
+        const frag pf = acc_frag<T>(s[u], p);
+#pragma unroll
+        for (int m = 0; m < MT; ++m) acc[m] = Elem<T>::mma(Tl::col(lv, wk * KT + 32 * u + KS * p, m, lane), pf, acc[m]);
+      }
+  }
+  l += other_half(l);
+  float mc = mx * a.c;   // -inf: no key seen
+
+  const long row_out = (long)bh * a.R + r;
+  T* const O = static_cast<T*>(a.o) + b * a.so.b + (hk * a.G + g) * a.so.h + t * a.so.t;
+  const long prow = ((long)bh * a.splits + split) * a.R;
+  float2* const part_ml = reinterpret_cast<float2*>(a.part + (long)a.B * a.Hkv * a.splits * a.R * a.D);
+  if constexpr (WK == 1) {
+    if (r >= a.R) return;
+    if (a.splits > 1) {
+      store_cols<float, MT>(a.part + (prow + r) * a.D, acc, 1.f, a.D, lane);
+      if (hi == 0) part_ml[prow + r] = float2{mc, l};
+    } else {
+      store_cols<T, MT>(O, acc, l == 0.f ? 0.f : 1.f / l, a.D, lane);
+      if (hi == 0) a.lse[row_out] = l == 0.f ? -inf() : (mc + __builtin_amdgcn_logf(l) - PShift<T>::log2) * kLn2;
+    }
+  } else {
+    static_assert(WQ == 1, "the waves that share rows are all four");
+    if (hi == 0) { ml[0][wk][lane] = mc; ml[1][wk][lane] = l; }
+    __syncthreads();   // also: the last tile has been read
+    float M = -inf(), L = 0.f;
+#pragma unroll
+    for (int w = 0; w < WK; ++w) M = fmaxf(M, ml[0][w][lane & 31]);
+    const float Mz = M == -inf() ? 0.f : M;
+#pragma unroll
+    for (int w = 0; w < WK; ++w) L += ml[1][w][lane & 31] * exp2_(ml[0][w][lane & 31] - Mz);
+    const float f = exp2_(mc - Mz) * (a.splits > 1 ? 1.f : L == 0.f ? 0.f : 1.f / L);
+    float* const red = reinterpret_cast<float*>(smem);
+    put_rows<DH>(red + wk * 32 * DH, acc, f, lane);
+    __syncthreads();
+    if (wave == 0 && hi == 0 && r < a.R) {
+      if (a.splits > 1) part_ml[prow + r] = float2{M, L};
+      else a.lse[row_out] = L == 0.f ? -inf() : (M + __builtin_amdgcn_logf(L) - PShift<T>::log2) * kLn2;
+    }
+    for (int i = threadIdx.x; i < 32 * (DH / 4); i += 256) {
+      const int row = i / (DH / 4), d = i % (DH / 4) * 4, rr = r0 + row;
+      if (rr >= a.R || d >= a.D) continue;
+      const f32x4 v = sum_rows<DH>(red, row, d);
+      if (a.splits > 1) *reinterpret_cast<f32x4*>(a.part + (prow + rr) * a.D + d) = v;
+      else {
+        const int gg = rr / a.Tq, tt = rr - gg * a.Tq;
+        store4<T>(static_cast<T*>(a.o) + b * a.so.b + (hk * a.G + gg) * a.so.h + tt * a.so.t + d, v[0], v[1], v[2], v[3]);
+      }
+    }
+  }
+}
+
+// splits of the keys joined: one wave per row, two channels a lane, in split order
+template <typename T> __global__ __launch_bounds__(256) void k_attn_join(AttnArgs a) {
+  const int lane = threadIdx.x & 63;
+  const long row = (long)blockIdx.x * 4 + (threadIdx.x >> 6);
+  if (row >= (long)a.B * a.Hkv * a.R) return;
+  const long bh = row / a.R, r = row - bh * a.R;
+  const float2* ml = reinterpret_cast<const float2*>(a.part + (long)a.B * a.Hkv * a.splits * a.R * a.D) + bh * a.splits * a.R + r;
+  float M = -inf(), L = 0.f, o0 = 0.f, o1 = 0.f;
+  for (int s = 0; s < a.splits; ++s) M = fmaxf(M, ml[(long)s * a.R].x);
+  const float Mz = M == -inf() ? 0.f : M;
+  for (int s = 0; s < a.splits; ++s) {
+    const float2 v = ml[(long)s * a.R];
+    const float w = exp2_(v.x - Mz);
+    L += v.y * w;
+    if (2 * lane < a.D) {
+      const float2 o = *reinterpret_cast<const float2*>(a.part + ((bh * a.splits + s) * a.R + r) * a.D + 2 * lane);
+      o0 += o.x * w;
+      o1 += o.y * w;
+    }
+  }
+  const float f = L == 0.f ? 0.f : 1.f / L;
+  const int b = (int)(bh / a.Hkv), hk = (int)(bh % a.Hkv), g = (int)r / a.Tq, t = (int)r - g * a.Tq;
+  if (2 * lane < a.D) {
+    T* p = static_cast<T*>(a.o) + b * a.so.b + (hk * a.G + g) * a.so.h + t * a.so.t + 2 * lane;
+    p[0] = (T)(o0 * f);
+    p[1] = (T)(o1 * f);
+  }
+  if (lane == 0) a.lse[row] = L == 0.f ? -inf() : (M + __builtin_amdgcn_logf(L) - PShift<T>::log2) * kLn2;
+}
+
+// ---------------------------------------------------------------------------------------------------------------- backward
+// fp16 only: dS can lie far below fp16's smallest normal number (6e-5) although do and the result do not.  Each lane's column of dS carries a
+// power of two that puts its largest element so far near 2^14; the accumulators carry the same factor and are moved along when it shrinks.
+struct RunScale {
+  float s = 0x1p100f;
+  template <int MT> __device__ inline void fit(f32x16& ds, f32x16* acc) {
+    float top = 0.f;
+#pragma unroll
+    for (int e = 0; e < 16; ++e) top = fmaxf(top, fabsf(ds[e]));
+    top = fmaxf(top, other_half(top));
+    const bool move = top * s > 0x1p15f;
+    if (__any(move)) {
+      const float n = move ? __builtin_ldexpf(1.f, 14 - (int)((__builtin_bit_cast(unsigned, top) >> 23) & 255) + 127) : s, f = n / s;
+      s = n;
+#pragma unroll
+      for (int m = 0; m < MT; ++m) acc[m] *= f;
+    }
+    ds *= s;
+  }
+};
+
+// dq, and delta for the dk / dv pass (which runs behind this one).  Same split of rows and keys over the waves as the forward.
+template <typename T, int DH, int WQ, int KT>
+__global__ __launch_bounds__(256) void k_attn_dq(AttnArgs a) {
+  typedef Tile<T, DH> Tl;
+  typedef typename Elem<T>::frag frag;
+  constexpr bool kScaled = DtOf<T>::v == DT_F16;
+  constexpr int KS = Elem<T>::KS, WK = 4 / WQ, TK = KT * WK, NS = DH / KS, MT = DH / 32, NU = KT / 32, NP = 32 / KS;
+  constexpr int kTile = TK * Tl::CPR, kMerge = WK > 1 ? WK * 32 * DH / 4 : 0;
+  __shared__ uint4 smem[2 * kTile > kMerge ? 2 * kTile : kMerge];
+  uint4 *const lk = smem, *const lv = smem + kTile;
+  int bh, tile, split;
+  decode(a, bh, tile, split);
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wq = wave / WK, wk = wave % WK, hi = lane >> 5;
+  const int b = bh / a.Hkv, hk = bh % a.Hkv;
+  const int r0 = tile * 32 * WQ, r = r0 + wq * 32 + (lane & 31), rc = min(r, a.R - 1), g = rc / a.Tq, t = rc - g * a.Tq;
+  const int h = hk * a.G + g;
+  const int kmax = key_end(a, r0, min(r0 + 32 * WQ, a.R) - 1), steps = (kmax + TK - 1) / TK;
+  const int lim = a.causal ? t + a.off : INT_MAX;
+  const T* const K = static_cast<const T*>(a.k) + b * a.sk.b + hk * a.sk.h;
+  const T* const V = static_cast<const T*>(a.v) + b * a.sv.b + hk * a.sv.h;
+  const uint8_t* const mask = a.mask ? a.mask + (long)b * a.Tk : nullptr;
+  frag qf[NS], gf[NS];
+  load_rows<T, DH>(qf, static_cast<const T*>(a.q) + b * a.sq.b + h * a.sq.h + t * a.sq.t, a.D, lane);
+  load_rows<T, DH>(gf, static_cast<const T*>(a.go) + b * a.sgo.b + h * a.sgo.h + t * a.sgo.t, a.D, lane);
+  const float lse = a.lse[(long)bh * a.R + rc];
+  const bool empty = lse == -inf();
+  float delta = 0.f;
+  {
+    frag of[NS];
+    load_rows<T, DH>(of, static_cast<const T*>(a.o) + b * a.so.b + h * a.so.h + t * a.so.t, a.D, lane);
+#pragma unroll
+    for (int s = 0; s < NS; ++s)
+#pragma unroll
+      for (int j = 0; j < Elem<T>::VEC; ++j) delta = __builtin_fmaf((float)gf[s][j], (float)of[s][j], delta);
+    delta += other_half(delta);
+    if (empty) delta = 0.f;   // (whatever stands in do there)
+  }
+  if (wk == 0 && hi == 0 && split == 0 && r < a.R) a.delta[(long)bh * a.R + r] = delta;
+  const float L = empty ? inf() : lse * kLog2e;   // exp2(x - inf) = 0
+  f32x16 acc[MT];
+#pragma unroll
+  for (int m = 0; m < MT; ++m) acc[m] = f32x16{0};
+  RunScale rs;
+
+  Stage<T, DH, TK> sk, sv;
+  unsigned long long bits_next = 0;
+  auto fetch = [&](int st) {
+    const int k0 = st * TK;
+    const int kk = k0 + wk * KT + lane;
+    bits_next = __ballot(lane < KT && kk < a.Tk && !(mask && mask[min(kk, a.Tk - 1)]));
+    auto ok = [&](int row) { const int key = k0 + row; return key < a.Tk && !(mask && mask[key]); };
+    sk.load([&](int row, int) { return ok(row) ? K + (long)(k0 + row) * a.sk.t : nullptr; }, a.D);
+    sv.load([&](int row, int) { return ok(row) ? V + (long)(k0 + row) * a.sv.t : nullptr; }, a.D);
+  };
+  if (split < steps) fetch(split);
+  for (int st = split; st < steps; st += a.splits) {
+    __syncthreads();
+    sk.store(lk);
+    sv.store(lv);
+    const unsigned long long bits = bits_next;
+    __syncthreads();
+    if (st + a.splits < steps) fetch(st + a.splits);
+    if (bits == 0) continue;
+    const int rel = lim - (st * TK + wk * KT);
+    const unsigned long long full = KT == 64 ? ~0ull : (1ull << KT) - 1;
+    const bool whole = __all(bits == full && rel >= KT - 1 && !empty);
+    const unsigned long long ok = empty ? 0ull : bits & (rel >= 63 ? ~0ull : rel < 0 ? 0ull : (2ull << rel) - 1);
+#pragma unroll
+    for (int u = 0; u < NU; ++u) {
+      f32x16 s = {0}, dp = {0};
+      const int kr = wk * KT + 32 * u;
+#pragma unroll
+      for (int i = 0; i < NS; ++i) {
+        s = Elem<T>::mma(Tl::row(lk, kr + (lane & 31), 2 * i + hi), qf[i], s);
+        dp = Elem<T>::mma(Tl::row(lv, kr + (lane & 31), 2 * i + hi), gf[i], dp);
+      }
+#pragma unroll
+      for (int e = 0; e < 16; ++e) s[e] = exp2_(__builtin_fmaf(s[e], a.c, -L)) * (dp[e] - delta);
+      if (!whole) {
+        const unsigned w = (unsigned)(ok >> (32 * u)) >> (4 * hi);
+#pragma unroll
+        for (int e = 0; e < 16; ++e) s[e] = (w >> (8 * (e >> 2) + (e & 3))) & 1 ? s[e] : 0.f;
+      }
+      if constexpr (kScaled) rs.fit<MT>(s, acc);
+#pragma unroll
+      for (int p = 0; p < NP; ++p) {
+        const frag df = acc_frag<T>(s, p);
+#pragma unroll
+        for (int m = 0; m < MT; ++m) acc[m] = Elem<T>::mma(Tl::col(lk, kr + KS * p, m, lane), df, acc[m]);
+      }
+    }
+  }
+  float f = a.scale;
+  if constexpr (kScaled) f /= rs.s;
+  const long prow = ((long)bh * a.splits + split) * a.R;
+  if constexpr (WK == 1) {
+    if (r >= a.R) return;
+    if (a.splits > 1) store_cols<float, MT>(a.part + (prow + r) * a.D, acc, f, a.D, lane);
+    else store_cols<T, MT>(static_cast<T*>(a.dq) + b * a.sdq.b + h * a.sdq.h + t * a.sdq.t, acc, f, a.D, lane);
+  } else {
+    __syncthreads();
+    float* const red = reinterpret_cast<float*>(smem);
+    put_rows<DH>(red + wk * 32 * DH, acc, f, lane);
+    __syncthreads();
+    for (int i = threadIdx.x; i < 32 * (DH / 4); i += 256) {
+      const int row = i / (DH / 4), d = i % (DH / 4) * 4, rr = r0 + row;
+      if (rr >= a.R || d >= a.D) continue;
+      const f32x4 v = sum_rows<DH>(red, row, d);
+      if (a.splits > 1) *reinterpret_cast<f32x4*>(a.part + (prow + rr) * a.D + d) = v;
+      else {
+        const int gg = rr / a.Tq, tt = rr - gg * a.Tq;
+        store4<T>(static_cast<T*>(a.dq) + b * a.sdq.b + (hk * a.G + gg) * a.sdq.h + tt * a.sdq.t + d, v[0], v[1], v[2], v[3]);
+      }
+    }
+  }
+}
+
+// partial sums [B * Hkv][splits][n rows][D] of one gradient joined in split order; rows are (g, t) with G = rows / T heads per kv head
+struct JoinArgs { const float* part; void* out; Str so; int Hkv, rows, T, D, splits; long nvec; };
+template <typename T> __global__ __launch_bounds__(256) void k_attn_join_sum(JoinArgs a) {
+  const long i = (long)blockIdx.x * 256 + threadIdx.x;
+  if (i >= a.nvec) return;
+  const int d4 = a.D / 4, d = (int)(i % d4) * 4;
+  const long row = i / d4, bh = row / a.rows;
+  const int r = (int)(row - bh * a.rows), G = a.rows / a.T, g = r / a.T, t = r - g * a.T;
+  f32x4 v = {0, 0, 0, 0};
+  for (int s = 0; s < a.splits; ++s) v += *reinterpret_cast<const f32x4*>(a.part + ((bh * a.splits + s) * a.rows + r) * a.D + d);
+  store4<T>(static_cast<T*>(a.out) + (bh / a.Hkv) * a.so.b + ((bh % a.Hkv) * G + g) * a.so.h + t * a.so.t + d, v[0], v[1], v[2], v[3]);
+}
+
+// dk, dv: WN waves own 32 keys each, the other factor (WR) shares those keys and takes RT rows each of every step
+template <typename T, int DH, int WN, int RT>
+__global__ __launch_bounds__(256) void k_attn_dkv(AttnArgs a) {
+  typedef Tile<T, DH> Tl;
+  typedef typename Elem<T>::frag frag;
+  constexpr bool kScaled = DtOf<T>::v == DT_F16;
+  constexpr int KS = Elem<T>::KS, WR = 4 / WN, TR = RT * WR, NS = DH / KS, MT = DH / 32, NU = RT / 32, NP = 32 / KS;
+  constexpr int kTile = TR * Tl::CPR, kMerge = WR > 1 ? WR * 32 * DH / 4 : 0;
+  __shared__ uint4 smem[2 * kTile > kMerge ? 2 * kTile : kMerge];
+  __shared__ __attribute__((aligned(16))) float rowL[TR], rowD[TR];
+  __shared__ __attribute__((aligned(16))) int rowK[TR];
+  uint4 *const lq = smem, *const lg = smem + kTile;
+  int bh, tile, split;
+  decode(a, bh, tile, split);
+  tile = a.tiles - 1 - tile;   // early keys are the long ones here
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wn = wave / WR, wr = wave % WR, hi = lane >> 5;
+  const int b = bh / a.Hkv, hk = bh % a.Hkv;
+  const int k0 = tile * 32 * WN, key = k0 + wn * 32 + (lane & 31);
+  const bool kok = key < a.Tk && !(a.mask && a.mask[(long)b * a.Tk + min(key, a.Tk - 1)]);
+  frag kf[NS], vf[NS];
+  load_rows<T, DH>(kf, kok ? static_cast<const T*>(a.k) + b * a.sk.b + hk * a.sk.h + (long)key * a.sk.t : nullptr, a.D, lane);
+  load_rows<T, DH>(vf, kok ? static_cast<const T*>(a.v) + b * a.sv.b + hk * a.sv.h + (long)key * a.sv.t : nullptr, a.D, lane);
+  f32x16 dk[MT], dv[MT];
+#pragma unroll
+  for (int m = 0; m < MT; ++m) dk[m] = dv[m] = f32x16{0};
+  RunScale rs;
+
+  const T* const Q = static_cast<const T*>(a.q) + b * a.sq.b + (long)hk * a.G * a.sq.h;
+  const T* const Go = static_cast<const T*>(a.go) + b * a.sgo.b + (long)hk * a.G * a.sgo.h;
+  const int steps = __syncthreads_or(kok) ? (a.R + TR - 1) / TR : 0;   // all keys masked: zeros
+  auto needed = [&](int st) {   // some row of the step sees some key of this tile
+    if (!a.causal) return true;
+    const int ra = st * TR, rb = min(ra + TR, a.R) - 1;
+    const int t = ra / a.Tq == rb / a.Tq ? rb % a.Tq : a.Tq - 1;
+    return t + a.off >= k0;
+  };
+  auto after = [&](int st) {
+    do st += a.splits; while (st < steps && !needed(st));
+    return st;
+  };
+  Stage<T, DH, TR> sq, sg;
+  float nL = 0.f, nD = 0.f;
+  int nK = 0;
+  auto fetch = [&](int st) {
+    const int r0 = st * TR;
+    auto where = [&](int row, const Str& s, const T* base) -> const T* {
+      const int r = r0 + row;
+      if (r >= a.R) return nullptr;
+      if (a.lse[(long)bh * a.R + r] == -inf()) return nullptr;   // a row that sees nothing: whatever stands in it stays out
+      const int g = a.G == 1 ? 0 : r / a.Tq;
+      return base + g * s.h + (long)(r - g * a.Tq) * s.t;
+    };
+    sq.load([&](int row, int) { return where(row, a.sq, Q); }, a.D);
+    sg.load([&](int row, int) { return where(row, a.sgo, Go); }, a.D);
+    if (threadIdx.x < TR) {
+      const int r = r0 + threadIdx.x;
+      nL = inf();
+      nD = 0.f;
+      nK = -1;
+      if (r < a.R) {
+        const float lse = a.lse[(long)bh * a.R + r];
+        nL = lse == -inf() ? inf() : lse * kLog2e;
+        nD = a.delta[(long)bh * a.R + r];
+        nK = a.causal ? (a.G == 1 ? r : r % a.Tq) + a.off : INT_MAX;
+      }
+    }
+  };
+  int st = split;
+  if (st < steps && !needed(st)) st = after(st);
+  if (st < steps) fetch(st);
+  while (st < steps) {
+    __syncthreads();
+    sq.store(lq);
+    sg.store(lg);
+    if (threadIdx.x < TR) { rowL[threadIdx.x] = nL; rowD[threadIdx.x] = nD; rowK[threadIdx.x] = nK; }
+    __syncthreads();
+    st = after(st);
+    if (st < steps) fetch(st);
+#pragma unroll
+    for (int u = 0; u < NU; ++u) {
+      f32x16 s = {0}, dp = {0};
+      const int rr = wr * RT + 32 * u;
+#pragma unroll
+      for (int i = 0; i < NS; ++i) {
+        s = Elem<T>::mma(Tl::row(lq, rr + (lane & 31), 2 * i + hi), kf[i], s);
+        dp = Elem<T>::mma(Tl::row(lg, rr + (lane & 31), 2 * i + hi), vf[i], dp);
+      }
+      f32x16 p;
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const int rq = rr + 8 * q + 4 * hi;
+        const f32x4 L = *reinterpret_cast<const f32x4*>(rowL + rq), dl = *reinterpret_cast<const f32x4*>(rowD + rq);
+        typedef int i32x4 __attribute__((ext_vector_type(4)));
+        const i32x4 kl = *reinterpret_cast<const i32x4*>(rowK + rq);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int e = 4 * q + i;
+          float x = exp2_(__builtin_fmaf(s[e], a.c, PShift<T>::log2 - L[i]));
+          if (a.causal) x = key <= kl[i] ? x : 0.f;
+          p[e] = x;
+          s[e] = x * PShift<T>::back * (dp[e] - dl[i]);
+        }
+      }
+      if constexpr (kScaled) rs.fit<MT>(s, dk);
+#pragma unroll
+      for (int i = 0; i < NP; ++i) {
+        const frag pf = acc_frag<T>(p, i), df = acc_frag<T>(s, i);
+#pragma unroll
+        for (int m = 0; m < MT; ++m) {
+          dv[m] = Elem<T>::mma(Tl::col(lg, rr + KS * i, m, lane), pf, dv[m]);
+          dk[m] = Elem<T>::mma(Tl::col(lq, rr + KS * i, m, lane), df, dk[m]);
+        }
+      }
+    }
+  }
+  float f = a.scale, fv = PShift<T>::back;
+  if constexpr (kScaled) f /= rs.s;
+  if (!kok) {   // a masked key: its column saw the row sums of the others
+    f = fv = 0.f;
+#pragma unroll
+    for (int m = 0; m < MT; ++m) dk[m] = dv[m] = f32x16{0};
+  }
+  const long prow = ((long)bh * a.splits + split) * a.Tk, pv = (long)a.B * a.Hkv * a.splits * a.Tk * a.D;
+  if constexpr (WR == 1) {
+    if (key >= a.Tk) return;
+    if (a.splits > 1) {
+      store_cols<float, MT>(a.part + (prow + key) * a.D, dk, f, a.D, lane);
+      store_cols<float, MT>(a.part + pv + (prow + key) * a.D, dv, fv, a.D, lane);
+    } else {
+      store_cols<T, MT>(static_cast<T*>(a.dk) + b * a.sdk.b + hk * a.sdk.h + (long)key * a.sdk.t, dk, f, a.D, lane);
+      store_cols<T, MT>(static_cast<T*>(a.dv) + b * a.sdv.b + hk * a.sdv.h + (long)key * a.sdv.t, dv, fv, a.D, lane);
+    }
+  } else {
+    float* const red = reinterpret_cast<float*>(smem);
+#pragma unroll
+    for (int which = 0; which < 2; ++which) {
+      __syncthreads();
+      put_rows<DH>(red + wr * 32 * DH, which ? dv : dk, which ? fv : f, lane);
+      __syncthreads();
+      for (int i = threadIdx.x; i < 32 * (DH / 4); i += 256) {
+        const int row = i / (DH / 4), d = i % (DH / 4) * 4, kk = k0 + row;
+        if (kk >= a.Tk || d >= a.D) continue;
+        const f32x4 v = sum_rows<DH>(red, row, d);
+        if (a.splits > 1) *reinterpret_cast<f32x4*>(a.part + which * pv + (prow + kk) * a.D + d) = v;
+        else if (which) store4<T>(static_cast<T*>(a.dv) + b * a.sdv.b + hk * a.sdv.h + (long)kk * a.sdv.t + d, v[0], v[1], v[2], v[3]);
+        else store4<T>(static_cast<T*>(a.dk) + b * a.sdk.b + hk * a.sdk.h + (long)kk * a.sdk.t + d, v[0], v[1], v[2], v[3]);
+      }
+    }
+  }
+}
+}  // namespace
+
+// ---------------------------------------------------------------------------------------------------------------- launches
+namespace {
+
+// How a pass is cut.  Four waves x 32 rows share every staged tile where that alone gives two workgroups per CU; below, 32-row workgroups
+// whose waves share the keys; and while even those leave CUs empty the other axis is split over workgroups and joined.
+struct Plan { int narrow, tiles, splits; };   // narrow: 32 rows per workgroup
+Plan plan_of(int nb, int rows, int across) {
+  Plan p;
+  const long n32 = (long)nb * ((rows + 31) / 32);
+  p.narrow = n32 <= 512;
+  p.tiles = p.narrow ? (rows + 31) / 32 : (rows + 127) / 128;
+  const long base = (long)nb * p.tiles;
+  const int steps = p.narrow ? (across + 127) / 128 : (across + 63) / 64;
+  long s = base >= 256 ? 1 : (512 + base - 1) / (base > 0 ? base : 1);
+  s = std::min<long>(s, steps / 2);
+  p.splits = (int)std::max<long>(1, std::min<long>(s, 64));
+  return p;
+}
+
+const char* check(const fdx_attn_desc* d) {
+  if (!d) return "null descriptor";
+  if (d->dtype < 0 || d->dtype > 2) return "dtype must be FDX_F32, FDX_BF16 or FDX_F16";
+  if (d->batch < 0 || d->heads <= 0 || d->kv_heads <= 0 || d->q_len < 0 || d->k_len < 0) return "negative size or no heads";
+  if (d->heads % d->kv_heads) return "heads must be a multiple of kv_heads";
+  if (d->head_dim <= 0 || d->head_dim > 128 || d->head_dim % 8) return "head_dim must be a multiple of 8 up to 128";
+  if (!(d->scale > 0.f) || !std::isfinite(d->scale)) return "scale must be positive and finite";
+  const long R = (long)(d->heads / d->kv_heads) * d->q_len, nb = (long)d->batch * d->kv_heads;
+  if (R > INT_MAX / 2 || d->k_len > INT_MAX / 2) return "too many rows for one key / value head";
+  if (nb * ((R + 31) / 32) > INT_MAX / 64 || nb * (((long)d->k_len + 31) / 32) > INT_MAX / 64) return "too many tiles for one launch";
+  return nullptr;
+}
+
+const char* check(const fdx_attn_desc* d, const fdx_bht* t, bool required) {
+  if (!t || !t->data) return required ? "null tensor" : nullptr;
+  const int vec = d->dtype == DT_F32 ? 4 : 8;
+  if ((reinterpret_cast<uintptr_t>(t->data) & 15) || t->b % vec || t->h % vec || t->t % vec) return "tensors must be 16-byte aligned, strides whole 16 bytes";
+  return nullptr;
+}
+
+AttnArgs args_of(const fdx_attn_desc* d) {
+  AttnArgs a{};
+  a.B = d->batch; a.H = d->heads; a.Hkv = d->kv_heads; a.G = d->heads / d->kv_heads;
+  a.Tq = d->q_len; a.Tk = d->k_len; a.D = d->head_dim; a.R = a.G * a.Tq;
+  a.off = a.Tk - a.Tq; a.causal = d->causal != 0;
+  a.scale = d->scale; a.c = d->scale * kLog2e;
+  return a;
+}
+Str str_of(const fdx_bht* t) { return t ? Str{(long)t->b, (long)t->h, (long)t->t} : Str{0, 0, 0}; }
+
+size_t fwd_floats(const fdx_attn_desc* d, Plan p) {
+  return p.splits > 1 ? (size_t)d->batch * d->heads * d->q_len * p.splits * (d->head_dim + 2) : 0;
+}
+size_t dq_floats(const fdx_attn_desc* d, Plan p) { return p.splits > 1 ? (size_t)d->batch * d->heads * d->q_len * p.splits * d->head_dim : 0; }
+size_t dkv_floats(const fdx_attn_desc* d, Plan p) { return p.splits > 1 ? (size_t)2 * d->batch * d->kv_heads * d->k_len * p.splits * d->head_dim : 0; }
+size_t delta_floats(const fdx_attn_desc* d) { return ((size_t)d->batch * d->heads * d->q_len + 3) / 4 * 4; }
+
+template <template <typename, int> class Run, typename... A> hipError_t by_type(const fdx_attn_desc* d, A&&... x) {
+  const int w = d->head_dim <= 32 ? 0 : d->head_dim <= 64 ? 1 : 2;
+  switch (d->dtype * 3 + w) {
+    case 0: return Run<float, 32>::go(x...);
+    case 1: return Run<float, 64>::go(x...);
+    case 2: return Run<float, 128>::go(x...);
+    case 3: return Run<bf16_t, 32>::go(x...);
+    case 4: return Run<bf16_t, 64>::go(x...);
+    case 5: return Run<bf16_t, 128>::go(x...);
+    case 6: return Run<f16_t, 32>::go(x...);
+    case 7: return Run<f16_t, 64>::go(x...);
+    default: return Run<f16_t, 128>::go(x...);
+  }
+}
+
+template <typename T, int DH> struct RunFwd {
+  static hipError_t go(AttnArgs& a, const Plan& p, hipStream_t s) {
+    a.tiles = p.tiles; a.splits = p.splits;
+    const unsigned grid = (unsigned)((long)a.B * a.Hkv * p.tiles * p.splits);
+    hipError_t e = p.narrow ? launch(k_attn_fwd<T, DH, 1, 32>, grid, 256, a, s) : launch(k_attn_fwd<T, DH, 4, 64>, grid, 256, a, s);
+    if (e == hipSuccess && p.splits > 1) e = launch(k_attn_join<T>, (unsigned)(((long)a.B * a.Hkv * a.R + 3) / 4), 256, a, s);
+    return e;
+  }
+};
+
+template <typename T, int DH> struct RunBwd {
+  static hipError_t join(const AttnArgs& a, const float* part, void* out, const Str& so, int rows, int T_, hipStream_t s) {
+    JoinArgs j{part, out, so, a.Hkv, rows, T_, a.D, a.splits, (long)a.B * a.Hkv * rows * (a.D / 4)};
+    return launch(k_attn_join_sum<T>, (unsigned)((j.nvec + 255) / 256), 256, j, s);
+  }
+  static hipError_t go(AttnArgs& a, const Plan& pq, const Plan& pk, float* part, hipStream_t s) {
+    hipError_t e = hipSuccess;
+    a.part = part;
+    if (a.R > 0) {
+      a.tiles = pq.tiles; a.splits = pq.splits;
+      const unsigned grid = (unsigned)((long)a.B * a.Hkv * pq.tiles * pq.splits);
+      e = pq.narrow ? launch(k_attn_dq<T, DH, 1, 32>, grid, 256, a, s) : launch(k_attn_dq<T, DH, 4, 64>, grid, 256, a, s);
+      if (e == hipSuccess && pq.splits > 1) e = join(a, part, a.dq, a.sdq, a.R, a.Tq, s);
+    }
+    if (e == hipSuccess && a.Tk > 0) {   // (reuses the partial sums' memory: ordered by the stream)
+      a.tiles = pk.tiles; a.splits = pk.splits;
+      const unsigned grid = (unsigned)((long)a.B * a.Hkv * pk.tiles * pk.splits);
+      e = pk.narrow ? launch(k_attn_dkv<T, DH, 1, 32>, grid, 256, a, s) : launch(k_attn_dkv<T, DH, 4, 64>, grid, 256, a, s);
+      if (e == hipSuccess && pk.splits > 1) {
+        const size_t half = (size_t)a.B * a.Hkv * a.splits * a.Tk * a.D;
+        e = join(a, part, a.dk, a.sdk, a.Tk, a.Tk, s);
+        if (e == hipSuccess) e = join(a, part + half, a.dv, a.sdv, a.Tk, a.Tk, s);
+      }
+    }
+    return e;
+  }
+};
+
+}  // namespace
+
+extern "C" int fdx_attn_forward_workspace(const fdx_attn_desc* d, size_t* bytes) {
+  if (const char* why = check(d)) return fail(nullptr, FDX_E_ARG, "fdx_attn_forward_workspace: %s", why);
+  if (!bytes) return fail(nullptr, FDX_E_ARG, "fdx_attn_forward_workspace: null size pointer");
+  const int rows = d->heads / d->kv_heads * d->q_len;
+  *bytes = fwd_floats(d, plan_of(d->batch * d->kv_heads, rows, d->k_len)) * sizeof(float);
+  return FDX_OK;
+}
+
+extern "C" int fdx_attn_backward_workspace(const fdx_attn_desc* d, size_t* bytes) {
+  if (const char* why = check(d)) return fail(nullptr, FDX_E_ARG, "fdx_attn_backward_workspace: %s", why);
+  if (!bytes) return fail(nullptr, FDX_E_ARG, "fdx_attn_backward_workspace: null size pointer");
+  const int rows = d->heads / d->kv_heads * d->q_len, nb = d->batch * d->kv_heads;
+  *bytes = (delta_floats(d) + std::max(dq_floats(d, plan_of(nb, rows, d->k_len)), dkv_floats(d, plan_of(nb, d->k_len, rows)))) * sizeof(float);
+  return FDX_OK;
+}
+
+extern "C" int fdx_attn_forward(fdx_handle h, const fdx_attn_desc* d, const fdx_bht* q, const fdx_bht* k, const fdx_bht* v, const uint8_t* key_mask,
+                                const fdx_bht* out, float* lse, void* workspace, size_t bytes, fdx_stream st) {
+  if (!h) return fail(nullptr, FDX_E_ARG, "fdx_attn_forward: null handle");
+  if (const char* why = check(d)) return fail(h, FDX_E_ARG, "fdx_attn_forward: %s", why);
+  if (d->batch == 0 || d->q_len == 0) return FDX_OK;
+  const bool keys = d->k_len > 0;
+  const struct { const fdx_bht* t; bool need; } all[] = {{q, true}, {k, keys}, {v, keys}, {out, true}};
+  for (const auto& x : all)
+    if (const char* why = check(d, x.t, x.need)) return fail(h, FDX_E_ARG, "fdx_attn_forward: %s", why);
+  if (!lse) return fail(h, FDX_E_ARG, "fdx_attn_forward: null lse");
+  AttnArgs a = args_of(d);
+  const Plan p = plan_of(a.B * a.Hkv, a.R, a.Tk);
+  if (bytes < fwd_floats(d, p) * sizeof(float) || (p.splits > 1 && !workspace))
+    return fail(h, FDX_E_ARG, "fdx_attn_forward: workspace of %zu bytes, %zu needed", bytes, fwd_floats(d, p) * sizeof(float));
+  a.q = q->data; a.k = k ? k->data : nullptr; a.v = v ? v->data : nullptr; a.o = out->data;
+  a.sq = str_of(q); a.sk = str_of(k); a.sv = str_of(v); a.so = str_of(out);
+  a.mask = key_mask; a.lse = lse; a.part = static_cast<float*>(workspace);
+  DeviceScope dev(h->device);
+  FDX_HIP(h, dev.err);
+  FDX_HIP(h, by_type<RunFwd>(d, a, p, as_stream(st)));
+  return FDX_OK;
+}
+
+extern "C" int fdx_attn_backward(fdx_handle h, const fdx_attn_desc* d, const fdx_bht* grad_out, const fdx_bht* q, const fdx_bht* k, const fdx_bht* v,
+                                 const fdx_bht* out, const float* lse, const uint8_t* key_mask, const fdx_bht* dq, const fdx_bht* dk,
+                                 const fdx_bht* dv, void* workspace, size_t bytes, fdx_stream st) {
+  if (!h) return fail(nullptr, FDX_E_ARG, "fdx_attn_backward: null handle");
+  if (const char* why = check(d)) return fail(h, FDX_E_ARG, "fdx_attn_backward: %s", why);
+  if (d->batch == 0 || (d->q_len == 0 && d->k_len == 0)) return FDX_OK;
+  const bool rows = d->q_len > 0, keys = d->k_len > 0;
+  const struct { const fdx_bht* t; bool need; } all[] = {{grad_out, rows}, {q, rows}, {out, rows}, {dq, rows}, {k, keys}, {v, keys}, {dk, keys}, {dv, keys}};
+  for (const auto& x : all)
+    if (const char* why = check(d, x.t, x.need)) return fail(h, FDX_E_ARG, "fdx_attn_backward: %s", why);
+  if (rows && !lse) return fail(h, FDX_E_ARG, "fdx_attn_backward: null lse");
+  AttnArgs a = args_of(d);
+  const Plan pq = plan_of(a.B * a.Hkv, a.R, a.Tk), pk = plan_of(a.B * a.Hkv, a.Tk, a.R);
+  const size_t need = (delta_floats(d) + std::max(dq_floats(d, pq), dkv_floats(d, pk))) * sizeof(float);
+  if (bytes < need || (need && !workspace)) return fail(h, FDX_E_ARG, "fdx_attn_backward: workspace of %zu bytes, %zu needed", bytes, need);
+  const auto data = [](const fdx_bht* t) { return t ? t->data : nullptr; };
+  a.q = data(q); a.k = data(k); a.v = data(v); a.go = data(grad_out); a.o = data(out);
+  a.dq = data(dq); a.dk = data(dk); a.dv = data(dv);
+  a.sq = str_of(q); a.sk = str_of(k); a.sv = str_of(v); a.sgo = str_of(grad_out); a.so = str_of(out);
+  a.sdq = str_of(dq); a.sdk = str_of(dk); a.sdv = str_of(dv);
+  a.mask = key_mask; a.lse = const_cast<float*>(lse); a.delta = static_cast<float*>(workspace);
+  DeviceScope dev(h->device);
+  FDX_HIP(h, dev.err);
+  FDX_HIP(h, by_type<RunBwd>(d, a, pq, pk, static_cast<float*>(workspace) + delta_floats(d), as_stream(st)));
+  return FDX_OK;
+}

@@ -411,6 +411,34 @@ int fdx_features_forward_svs(fdx_handle h, const float* contents, int B, int S, 
 int fdx_repeat_expand(fdx_handle h, const float* src, long rows, int S, int T, float* dst, fdx_stream s);
 
 /* ------------------------------------------------------------------------------------------------
+ * Operators for training a denoiser (TransformerDecoderDenoiser.training_forward, modules/convnext.py:263-379: nn.TransformerDecoderLayer
+ * under autograd).  Stateless: nothing is kept in the handle between calls; partial sums live in a workspace of the caller's, whose size the
+ * *_workspace functions give (16-byte aligned; one per call in flight).  No atomics: the same inputs give the same bits.
+ * ---------------------------------------------------------------------------------------------- */
+enum { FDX_F32 = 0, FDX_BF16 = 1, FDX_F16 = 2 };
+/* A [batch][heads][length][channels] tensor, channels contiguous, the other strides in elements.  data 16-byte aligned, strides whole 16 bytes. */
+typedef struct { void* data; long long b, h, t; } fdx_bht;
+typedef struct fdx_attn_desc {
+  int dtype;                 /* FDX_F32 | FDX_BF16 | FDX_F16: q, k, v, out and their gradients; scores and sums are fp32 */
+  int batch, heads, kv_heads;/* heads a multiple of kv_heads: query head h reads kv head h / (heads / kv_heads) */
+  int q_len, k_len;          /* 0 allowed */
+  int head_dim;              /* multiple of 8, at most 128 */
+  int causal;                /* query i sees keys j <= i + k_len - q_len */
+  float scale;               /* > 0 */
+} fdx_attn_desc;
+/* out = softmax(scale q k^T) v; key_mask dev [batch][k_len] bytes, 1 = masked, or NULL: masked keys and values are never used, whatever they
+ * hold.  lse: dev fp32 [batch][heads][q_len], the natural logarithm of every row's sum of exponentials.  A row that sees no key: out 0, lse -inf. */
+int fdx_attn_forward_workspace(const fdx_attn_desc* d, size_t* bytes);
+int fdx_attn_forward(fdx_handle h, const fdx_attn_desc* d, const fdx_bht* q, const fdx_bht* k, const fdx_bht* v, const uint8_t* key_mask,
+                     const fdx_bht* out, float* lse, void* workspace, size_t bytes, fdx_stream s);
+/* Gradients from grad_out and the forward's out and lse; the probabilities are computed again.  Gradients of shared kv heads are summed over
+ * the query heads, those of masked keys are 0, those of a row that sees no key are 0 whatever grad_out holds there. */
+int fdx_attn_backward_workspace(const fdx_attn_desc* d, size_t* bytes);
+int fdx_attn_backward(fdx_handle h, const fdx_attn_desc* d, const fdx_bht* grad_out, const fdx_bht* q, const fdx_bht* k, const fdx_bht* v,
+                      const fdx_bht* out, const float* lse, const uint8_t* key_mask, const fdx_bht* dq, const fdx_bht* dk, const fdx_bht* dv,
+                      void* workspace, size_t bytes, fdx_stream s);
+
+/* ------------------------------------------------------------------------------------------------
  * Kernel-level test / profiling hooks (used by tests/ and bench.py only)
  * ---------------------------------------------------------------------------------------------- */
 /* y = conv1d(act_in(x), w) + bias with "same" zero padding: x dev [B][Cin][T], w HOST [Cout][Cin][k],
