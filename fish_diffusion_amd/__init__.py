@@ -12,9 +12,11 @@ from .diffsinger import ENCODERS, DiffSinger, NaiveProjectionEncoder, pitch_to_s
 from .refinegan import RefineGAN, RefineGANGenerator  # noqa: F401
 from .hifisinger import HiFiSinger  # noqa: F401
 from .inference import SVCModel, inference_model, load_checkpoint  # noqa: F401
-from .ops import attention, attention_backward, attention_forward  # noqa: F401
+from .ops import (attention, attention_backward, attention_forward, residual_norm, residual_norm_backward, residual_norm_forward,  # noqa: F401
+                  Packed8, pack8, unpack8, linear8, linear8_weight_grad, gelu8, gelu8_backward, gelu8_forward)
 from . import segments  # noqa: F401
 
 __all__ = ["DENOISERS", "DIFFUSIONS", "VOCODERS", "install", "WaveNet", "ConvNext", "TransformerDecoderDenoiser", "GaussianDiffusion", "NsfHifiGAN", "Generator",
            "PitchAdjustableMelSpectrogram", "ENCODERS", "DiffSinger", "NaiveProjectionEncoder", "pitch_to_scale", "repeat_expand", "RefineGAN", "RefineGANGenerator", "HiFiSinger", "SVCModel", "load_checkpoint", "inference_model",
-           "attention", "attention_forward", "attention_backward"]
+           "attention", "attention_forward", "attention_backward", "residual_norm", "residual_norm_forward", "residual_norm_backward",
+           "Packed8", "pack8", "unpack8", "linear8", "linear8_weight_grad", "gelu8", "gelu8_forward", "gelu8_backward"]

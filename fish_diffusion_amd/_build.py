@@ -15,7 +15,7 @@ from concurrent.futures import ThreadPoolExecutor
 HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 LIB = os.path.join(CSRC, "libfishdx.so")
-SOURCES = ["core.hip", "wavenet.hip", "nsf.hip", "mel.hip", "features.hip", "refinegan.hip", "convnext.hip", "tfdec.hip", "attention.hip"]
+SOURCES = ["core.hip", "wavenet.hip", "nsf.hip", "mel.hip", "features.hip", "refinegan.hip", "convnext.hip", "tfdec.hip", "attention.hip", "resnorm.hip", "pack8.hip"]
 # every header under csrc/ (+ the C ABI): a change to any of them rebuilds every object (a hand-kept list went stale once: a header-only fix
 # of the fused ResBlock kernel did not rebuild nsf.o)
 HEADERS = sorted(f for f in os.listdir(CSRC) if f.endswith(".h")) + ["../../include/fishdx.h"]

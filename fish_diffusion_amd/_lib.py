@@ -75,6 +75,11 @@ class AttnDesc(C.Structure):
     _fields_ = [(n, C.c_int) for n in ("dtype", "batch", "heads", "kv_heads", "q_len", "k_len", "head_dim", "causal")] + [("scale", C.c_float)]
 
 
+class ResnormDesc(C.Structure):
+    _fields_ = [("dtype", C.c_int), ("param_dtype", C.c_int), ("gate_dtype", C.c_int), ("rows", C.c_longlong), ("channels", C.c_int),
+                ("gate_rows", C.c_longlong), ("rms", C.c_int), ("residual_scale", C.c_float), ("eps", C.c_float)]
+
+
 DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 
 _P = C.c_void_p
@@ -128,6 +133,15 @@ _SIGS = {
     "fdx_attn_forward": (C.c_int, [_P, C.POINTER(AttnDesc), C.POINTER(Bht), C.POINTER(Bht), C.POINTER(Bht), _P, C.POINTER(Bht), _P, _P, C.c_size_t, _P]),
     "fdx_attn_backward_workspace": (C.c_int, [C.POINTER(AttnDesc), C.POINTER(C.c_size_t)]),
     "fdx_attn_backward": (C.c_int, [_P, C.POINTER(AttnDesc)] + [C.POINTER(Bht)] * 5 + [_P, _P] + [C.POINTER(Bht)] * 3 + [_P, C.c_size_t, _P]),
+    "fdx_resnorm_forward": (C.c_int, [_P, C.POINTER(ResnormDesc)] + [_P] * 11),
+    "fdx_resnorm_backward_workspace": (C.c_int, [C.POINTER(ResnormDesc), C.POINTER(C.c_size_t)]),
+    "fdx_resnorm_backward": (C.c_int, [_P, C.POINTER(ResnormDesc)] + [_P] * 18 + [C.c_size_t, _P]),
+    "fdx_pack8": (C.c_int, [_P, C.c_int, _P, C.c_longlong, C.c_int, _P, _P, _P]),
+    "fdx_unpack8": (C.c_int, [_P, C.c_int, _P, _P, C.c_longlong, C.c_int, _P, _P]),
+    "fdx_gelu8_forward": (C.c_int, [_P, C.c_int, _P, C.c_longlong, C.c_int, _P, _P, _P, _P]),
+    "fdx_gelu8_backward": (C.c_int, [_P, C.c_int, _P, _P, _P, C.c_longlong, C.c_int, _P, _P]),
+    "fdx_linear8_weight_grad_workspace": (C.c_int, [C.c_int, C.c_longlong, C.c_int, C.c_int, C.POINTER(C.c_size_t)]),
+    "fdx_linear8_weight_grad": (C.c_int, [_P, C.c_int, _P, _P, _P, C.c_longlong, C.c_int, C.c_int, C.c_int, _P, _P, _P, C.c_size_t, _P]),
     "fdx_bcast_arena": (C.c_int, [_P, C.c_size_t, _P, C.c_int, _P]),
     "fdx_refinegan_num_weights": (C.c_int, [C.POINTER(RefineGanDesc)]),
     "fdx_refinegan_num_noises": (C.c_int, [C.POINTER(RefineGanDesc)]),

@@ -3,6 +3,10 @@ fish_diffusion/modules/convnext.py:263-379) needs besides plain matrix products.
 
   attention / attention_forward / attention_backward
         softmax(scale q k^T) v with key masks, causal order and shared key / value heads; the backward pass recomputes the probabilities.
+  residual_norm / residual_norm_forward / residual_norm_backward
+        h = a x + gate * post_norm(block), y = pre_norm(h): the step between two blocks, one launch each way.
+  linear8, gelu8 (pack8, unpack8, linear8_weight_grad, gelu8_forward, gelu8_backward)
+        a linear layer and a GELU that keep their input in 8 bits; the gradients are taken straight from the 8-bit form.
 
 Each comes as a differentiable function and as the two calls it is made of (`*_forward`, `*_backward`); the latter build no autograd graph and
 may be captured into a HIP graph as they are.  Device tensors only (fp32, bf16, fp16); work runs on the current stream of the tensors' device and
@@ -12,7 +16,7 @@ from __future__ import annotations
 
 import ctypes as C
 import math
-from typing import Optional
+from typing import NamedTuple, Optional
 
 import torch
 from torch.autograd.function import once_differentiable
@@ -196,3 +200,317 @@ class _Attention(torch.autograd.Function):
 def attention(q, k, v, key_mask=None, causal=False, scale=None):
     """Differentiable `attention_forward`: returns out alone."""
     return _apply(_Attention, q, k, v, key_mask, causal, scale)
+
+
+# ------------------------------------------------------------------------------------------------------------- norm, gate, residual
+class ResidualNormGrads(NamedTuple):
+    """Gradients of `residual_norm_forward`'s arguments; None where the argument was None."""
+    dx: torch.Tensor
+    dblock: torch.Tensor
+    dgate: Optional[torch.Tensor]
+    dpost_weight: Optional[torch.Tensor]
+    dpost_bias: Optional[torch.Tensor]
+    dpre_weight: Optional[torch.Tensor]
+    dpre_bias: Optional[torch.Tensor]
+
+
+_KINDS = {"layer": 0, "rms": 1}
+
+
+def _packed_rows(t: Optional[torch.Tensor]) -> Optional[torch.Tensor]:
+    """Contiguous and 16-byte aligned (a copy where it is not)."""
+    if t is None or t.numel() == 0:
+        return t
+    t = t.contiguous()
+    return t if t.data_ptr() % 16 == 0 else t.clone()
+
+
+def _norm_args(x, block, gate, residual_scale, post_norm, pre_norm, kind, eps, what):
+    if not torch.is_tensor(x) or not torch.is_tensor(block) or x.dim() < 1 or x.shape != block.shape:
+        raise ValueError(f"{what}: x and block must be tensors of one shape [..., channels]")
+    dt = _dtype(x, what)
+    C_ = x.shape[-1]
+    if not 1 <= C_ <= 8192:
+        raise ValueError(f"{what}: {C_} channels are not within 1 ... 8192")
+    if kind not in _KINDS:
+        raise ValueError(f"{what}: kind must be 'layer' or 'rms', got {kind!r}")
+    if not (math.isfinite(residual_scale) and eps >= 0.0 and math.isfinite(eps)):
+        raise ValueError(f"{what}: residual_scale must be finite and eps finite and not negative")
+    params = []
+    for name, wb in (("post_norm", post_norm), ("pre_norm", pre_norm)):
+        w, b = (None, None) if wb is None else wb
+        if wb is not None and w is None:
+            raise ValueError(f"{what}: {name} must be (weight, bias or None)")
+        params += [w, b]
+    pdt = {p.dtype for p in params if p is not None} or {x.dtype}
+    if len(pdt) > 1 or not pdt <= {x.dtype, torch.float32}:
+        raise ValueError(f"{what}: the norms' weights and biases must all be {x.dtype} or all float32, got {sorted(map(str, pdt))}")
+    for p in params:
+        if p is not None and p.shape != (C_,):
+            raise ValueError(f"{what}: a norm's weight / bias has shape {tuple(p.shape)}, expected {(C_,)}")
+    N = x.numel() // C_
+    rows = 0
+    if gate is not None:
+        if gate.dtype not in (x.dtype, torch.float32):
+            raise ValueError(f"{what}: gate must be {x.dtype} or float32, got {gate.dtype}")
+        if gate.shape == x.shape and x.dim() > 1:
+            rows = 1
+        elif gate.shape == (C_,):
+            rows = max(N, 1)
+        elif x.dim() == 3 and tuple(gate.shape) in ((x.shape[0], C_), (x.shape[0], 1, C_)):
+            rows = max(x.shape[1], 1)
+        else:
+            raise ValueError(f"{what}: gate {tuple(gate.shape)} is none of [channels], [batch, channels], [batch, 1, channels] and x's {tuple(x.shape)}")
+    for name, t in (("x", x), ("block", block), ("gate", gate), ("a norm's weight or bias", next((p for p in params if p is not None), None))):
+        if t is not None:
+            _lib.require_gpu(t, f"{what} {name}")
+    for t in (block, gate, *params):
+        if t is not None and t.device != x.device:
+            raise ValueError(f"{what}: tensors on {t.device} and {x.device}")
+    if block.dtype != x.dtype:
+        raise ValueError(f"{what}: block is {block.dtype}, x {x.dtype}")
+    desc = _lib.ResnormDesc(dt, _lib.DTYPES[next(iter(pdt))], dt if gate is None else _lib.DTYPES[gate.dtype], N, C_, rows, _KINDS[kind],
+                            float(residual_scale), float(eps))
+    return desc, [_packed_rows(p) for p in params]
+
+
+@torch.no_grad()
+def residual_norm_forward(x, block, gate=None, residual_scale=1.0, post_norm=None, pre_norm=None, kind="layer", eps=1e-5):
+    """(h, y, stats): h = residual_scale * x + gate * post_norm(block), y = pre_norm(h) (None without one), stats for the backward pass.
+
+    x, block [..., C], C up to 8192; post_norm / pre_norm = (weight, bias or None) of a LayerNorm (kind "layer") or RMSNorm ("rms") over the last
+    dimension, or None; gate None, [C], x's own shape, or for x [B, T, C] one row per item: [B, C] or [B, 1, C].  Weights, biases and gate may be fp32
+    beside 16-bit x.  y is computed from h before h is rounded.  A post-norm block's x = norm(x + block) is pre_norm alone, its result y."""
+    desc, (pw, pb, nw, nb) = _norm_args(x, block, gate, residual_scale, post_norm, pre_norm, kind, eps, "residual_norm")
+    x, block, gate = _packed_rows(x), _packed_rows(block), _packed_rows(gate)
+    h_out = torch.empty_like(x)
+    y = torch.empty_like(x) if nw is not None else None
+    stats = torch.empty((*x.shape[:-1], 4), dtype=torch.float32, device=x.device)
+    if x.numel():
+        h, lib = _handle(x.device), _lib.lib()
+        with h.lock:
+            _lib.check(lib.fdx_resnorm_forward(h.h, C.byref(desc), *(_lib.ptr(t) for t in (x, block, gate, pw, pb, nw, nb, h_out, y, stats)),
+                                               _lib.stream_ptr(x.device)), h.h)
+    return h_out, y, stats
+
+
+@torch.no_grad()
+def residual_norm_backward(grad_h, grad_y, x, block, stats, gate=None, residual_scale=1.0, post_norm=None, pre_norm=None, kind="layer", eps=1e-5):
+    """`ResidualNormGrads` from the gradients of h and y (either may be None) and the forward's arguments and stats.  Where there is no gate, no post norm and
+    residual_scale is 1, dx and dblock are equal and are ONE tensor.  The gate's gradient has the gate's shape."""
+    desc, (pw, pb, nw, nb) = _norm_args(x, block, gate, residual_scale, post_norm, pre_norm, kind, eps, "residual_norm_backward")
+    for name, g in (("grad_h", grad_h), ("grad_y", grad_y)):
+        if g is not None and (g.shape != x.shape or g.dtype != x.dtype or g.device != x.device):
+            raise ValueError(f"residual_norm_backward: {name} must be {x.dtype} {tuple(x.shape)} on {x.device}")
+    if grad_y is not None and nw is None:
+        raise ValueError("residual_norm_backward: grad_y without a pre_norm")
+    if stats.shape != (*x.shape[:-1], 4) or stats.dtype != torch.float32 or stats.device != x.device:
+        raise ValueError("residual_norm_backward: stats are not the forward's")
+    x, block, gate_c, grad_h, grad_y, stats = (_packed_rows(t) for t in (x, block, gate, grad_h, grad_y, stats))
+    dx = torch.empty_like(x)
+    dblock = dx if gate is None and pw is None and residual_scale == 1.0 else torch.empty_like(x)
+    dgate = None if gate is None else torch.empty_like(gate_c)
+    grads = [None if p is None else torch.empty_like(p) for p in (pw, pb, nw, nb)]
+    if x.numel() == 0:
+        for t in (dgate, *grads):
+            if t is not None:
+                t.zero_()
+    else:
+        h, lib = _handle(x.device), _lib.lib()
+        ws, n = _workspace(lib.fdx_resnorm_backward_workspace, desc, x.device)
+        with h.lock:
+            _lib.check(lib.fdx_resnorm_backward(h.h, C.byref(desc), *(_lib.ptr(t) for t in (grad_h, grad_y, x, block, gate_c, pw, pb, nw, nb, stats, dx, dblock,
+                                                                                           dgate, *grads, ws)), n, _lib.stream_ptr(x.device)), h.h)
+    return ResidualNormGrads(dx, dblock, dgate, *grads)
+
+
+class _ResidualNorm(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, block, gate, post_w, post_b, pre_w, pre_b, residual_scale, kind, eps):
+        post, pre = (None if w is None else (w, b) for w, b in ((post_w, post_b), (pre_w, pre_b)))
+        h, y, stats = residual_norm_forward(x, block, gate, residual_scale, post, pre, kind, eps)
+        ctx.save_for_backward(x, block, gate, post_w, post_b, pre_w, pre_b, stats)
+        ctx.rest = (residual_scale, kind, eps)
+        ctx.set_materialize_grads(False)
+        return h, y
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, grad_h, grad_y):
+        x, block, gate, post_w, post_b, pre_w, pre_b, stats = ctx.saved_tensors
+        residual_scale, kind, eps = ctx.rest
+        post, pre = (None if w is None else (w, b) for w, b in ((post_w, post_b), (pre_w, pre_b)))
+        return (*residual_norm_backward(grad_h, grad_y, x, block, stats, gate, residual_scale, post, pre, kind, eps), None, None, None)
+
+
+def residual_norm(x, block, gate=None, residual_scale=1.0, post_norm=None, pre_norm=None, kind="layer", eps=1e-5):
+    """Differentiable `residual_norm_forward`: returns (h, y)."""
+    return _apply(_ResidualNorm, x, block, gate, *(post_norm or (None, None)), *(pre_norm or (None, None)), residual_scale, kind, eps)
+
+
+# ------------------------------------------------------------------------------------------------------------- activations in 8 bits
+class Packed8(NamedTuple):
+    """A tensor [..., C] in 8 bits: codes int8 [..., C] and exponents uint8 [..., ceil(C / 32)]; a group of 32 channels shares 2 ** (exponent - 127)."""
+    codes: torch.Tensor
+    exponents: torch.Tensor
+
+
+def _rows_of(t: torch.Tensor, what: str, name: str):
+    if not torch.is_tensor(t) or t.dim() < 1 or t.shape[-1] < 1:
+        raise ValueError(f"{what}: {name} must be a [..., channels] tensor")
+    return t.numel() // t.shape[-1], t.shape[-1]
+
+
+def _packed_ok(p: Packed8, what: str) -> Packed8:
+    codes, exps = p
+    if not torch.is_tensor(codes) or codes.dtype != torch.int8 or exps.dtype != torch.uint8 or codes.dim() < 1 or codes.shape[-1] < 1:
+        raise ValueError(f"{what}: not a Packed8 of int8 codes and uint8 exponents")
+    if exps.shape != (*codes.shape[:-1], (codes.shape[-1] + 31) // 32):
+        raise ValueError(f"{what}: exponents {tuple(exps.shape)} do not belong to codes {tuple(codes.shape)}")
+    _lib.require_gpu(codes, f"{what} codes")
+    if exps.device != codes.device:
+        raise ValueError(f"{what}: codes on {codes.device}, exponents on {exps.device}")
+    return Packed8(_packed_rows(codes), exps.contiguous())
+
+
+def _new_packed(x: torch.Tensor) -> Packed8:
+    return Packed8(torch.empty(x.shape, dtype=torch.int8, device=x.device),
+                   torch.empty((*x.shape[:-1], (x.shape[-1] + 31) // 32), dtype=torch.uint8, device=x.device))
+
+
+@torch.no_grad()
+def pack8(x) -> Packed8:
+    """x [..., C] in 8 bits.  Each group of 32 channels shares the smallest power of two 2^k, k >= -126, with max|x| <= 127 * 2^k; codes are x / 2^k rounded to
+    nearest even, so the error is at most half of 2^k (at the very top of fp32's range, k = 122, codes end at 63 so that no finite value reads back
+    infinite).  A group with an infinity or NaN reads back as NaN."""
+    N, C_ = _rows_of(x, "pack8", "x")
+    dt = _dtype(x, "pack8")
+    _lib.require_gpu(x, "pack8 x")
+    x = _packed_rows(x)
+    p = _new_packed(x)
+    h = _handle(x.device)
+    with h.lock:
+        _lib.check(_lib.lib().fdx_pack8(h.h, dt, _lib.ptr(x), N, C_, _lib.ptr(p.codes), _lib.ptr(p.exponents), _lib.stream_ptr(x.device)), h.h)
+    return p
+
+
+@torch.no_grad()
+def unpack8(packed: Packed8, dtype=torch.float32) -> torch.Tensor:
+    """What the codes stand for (exact in float32 and bfloat16; in float16 at most 65504)."""
+    p = _packed_ok(packed, "unpack8")
+    if dtype not in _lib.DTYPES:
+        raise TypeError(f"unpack8: {dtype} is not one of float32, bfloat16, float16")
+    out = torch.empty(p.codes.shape, dtype=dtype, device=p.codes.device)
+    h = _handle(out.device)
+    with h.lock:
+        _lib.check(_lib.lib().fdx_unpack8(h.h, _lib.DTYPES[dtype], _lib.ptr(p.codes), _lib.ptr(p.exponents), *_rows_of(p.codes, "unpack8", "codes"), _lib.ptr(out),
+                                          _lib.stream_ptr(out.device)), h.h)
+    return out
+
+
+@torch.no_grad()
+def linear8_weight_grad(dy, packed: Packed8, bias=True, dtype=None):
+    """(dw, db) of y = x w^T + b from dy [..., out] and x kept as `pack8(x)` [..., in]: dw [out, in] = sum over rows of dy x8, db [out] = sum of dy (None if not
+    `bias`).  Products are exact and summed in fp32; results in `dtype` (default dy's)."""
+    N, O = _rows_of(dy, "linear8_weight_grad", "dy")
+    dt = _dtype(dy, "linear8_weight_grad")
+    dtype = dy.dtype if dtype is None else dtype
+    if dtype not in _lib.DTYPES:
+        raise TypeError(f"linear8_weight_grad: {dtype} is not one of float32, bfloat16, float16")
+    if packed.codes.shape[:-1] != dy.shape[:-1]:
+        raise ValueError(f"linear8_weight_grad: dy {tuple(dy.shape)} and the packed input {tuple(packed.codes.shape)} have different rows")
+    _lib.require_gpu(dy, "linear8_weight_grad dy")
+    p = _packed_ok(packed, "linear8_weight_grad")
+    if p.codes.device != dy.device:
+        raise ValueError(f"linear8_weight_grad: dy on {dy.device}, packed input on {p.codes.device}")
+    I = p.codes.shape[-1]
+    dy = _packed_rows(dy)
+    dw = torch.empty(O, I, dtype=dtype, device=dy.device)
+    db = torch.empty(O, dtype=dtype, device=dy.device) if bias else None
+    h, lib, n = _handle(dy.device), _lib.lib(), C.c_size_t()
+    _lib.check(lib.fdx_linear8_weight_grad_workspace(dt, N, O, I, C.byref(n)))
+    ws = torch.empty(n.value, dtype=torch.uint8, device=dy.device)
+    with h.lock:
+        _lib.check(lib.fdx_linear8_weight_grad(h.h, dt, _lib.ptr(dy), _lib.ptr(p.codes), _lib.ptr(p.exponents), N, O, I, _lib.DTYPES[dtype], _lib.ptr(dw),
+                                               _lib.ptr(db), _lib.ptr(ws), n.value, _lib.stream_ptr(dy.device)), h.h)
+    return dw, db
+
+
+@torch.no_grad()
+def gelu8_forward(x):
+    """(gelu(x), pack8(x)) in one pass; GELU in its erf form, from x itself."""
+    N, C_ = _rows_of(x, "gelu8", "x")
+    dt = _dtype(x, "gelu8")
+    _lib.require_gpu(x, "gelu8 x")
+    x = _packed_rows(x)
+    y, p = torch.empty_like(x), _new_packed(x)
+    h = _handle(x.device)
+    with h.lock:
+        _lib.check(_lib.lib().fdx_gelu8_forward(h.h, dt, _lib.ptr(x), N, C_, _lib.ptr(y), _lib.ptr(p.codes), _lib.ptr(p.exponents), _lib.stream_ptr(x.device)), h.h)
+    return y, p
+
+
+@torch.no_grad()
+def gelu8_backward(dy, packed: Packed8):
+    """dy * gelu'(x8), x8 what `packed` stands for."""
+    N, C_ = _rows_of(dy, "gelu8_backward", "dy")
+    dt = _dtype(dy, "gelu8_backward")
+    if packed.codes.shape != dy.shape:
+        raise ValueError(f"gelu8_backward: dy {tuple(dy.shape)} and the packed input {tuple(packed.codes.shape)} differ")
+    _lib.require_gpu(dy, "gelu8_backward dy")
+    p = _packed_ok(packed, "gelu8_backward")
+    if p.codes.device != dy.device:
+        raise ValueError(f"gelu8_backward: dy on {dy.device}, packed input on {p.codes.device}")
+    dy = _packed_rows(dy)
+    dx = torch.empty_like(dy)
+    h = _handle(dy.device)
+    with h.lock:
+        _lib.check(_lib.lib().fdx_gelu8_backward(h.h, dt, _lib.ptr(dy), _lib.ptr(p.codes), _lib.ptr(p.exponents), N, C_, _lib.ptr(dx), _lib.stream_ptr(dy.device)), h.h)
+    return dx
+
+
+class _Linear8(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, bias):
+        ctx.save_for_backward(*pack8(x), weight)
+        ctx.has_bias = bias is not None
+        return torch.nn.functional.linear(x, weight, bias)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy):
+        codes, exps, weight = ctx.saved_tensors
+        need_x, need_w, need_b = ctx.needs_input_grad
+        dx = torch.matmul(dy, weight) if need_x else None
+        dw, db = linear8_weight_grad(dy, Packed8(codes, exps), ctx.has_bias) if need_w or need_b else (None, None)
+        return dx, dw, db
+
+
+def linear8(x, weight, bias=None):
+    """Differentiable x weight^T + bias that keeps x in 8 bits for the weight's gradient (x, weight and bias of one type); the result itself and x's gradient
+    are those of torch.nn.functional.linear."""
+    N, I = _rows_of(x, "linear8", "x")
+    _dtype(x, "linear8")
+    if weight.dim() != 2 or weight.shape[1] != I or (bias is not None and bias.shape != weight.shape[:1]):
+        raise ValueError(f"linear8: x {tuple(x.shape)}, weight {tuple(weight.shape)} and bias do not fit together")
+    _lib.require_gpu(x, "linear8 x")
+    _same(x, "linear8", weight=weight, bias=bias)
+    return _apply(_Linear8, x, weight, bias)
+
+
+class _Gelu8(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x):
+        y, p = gelu8_forward(x)
+        ctx.save_for_backward(*p)
+        return y
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy):
+        return gelu8_backward(dy, Packed8(*ctx.saved_tensors))
+
+
+def gelu8(x):
+    """Differentiable GELU (erf form) that keeps its input in 8 bits for the backward pass."""
+    return _apply(_Gelu8, x)

@@ -438,6 +438,44 @@ int fdx_attn_backward(fdx_handle h, const fdx_attn_desc* d, const fdx_bht* grad_
                       const fdx_bht* out, const float* lse, const uint8_t* key_mask, const fdx_bht* dq, const fdx_bht* dk, const fdx_bht* dv,
                       void* workspace, size_t bytes, fdx_stream s);
 
+/* The step between two blocks: n = post(block), h = residual_scale x + gate n, y = pre(h) with post / pre LayerNorm or RMSNorm (weights given), or
+ * nothing (NULL weights; bias NULL: none).  All tensors dev, [rows][channels] contiguous; gate [rows / gate_rows][channels]: gate_rows = rows is one
+ * gate per channel, rows of an item one per item, 1 one per element, 0 no gate (NULL).  stats: dev fp32 [rows][4] for the backward pass, or NULL. */
+typedef struct fdx_resnorm_desc {
+  int dtype, param_dtype, gate_dtype;   /* x, block, h, y and gradients; the norms' weights and biases; the gate: the latter two dtype or FDX_F32 */
+  long long rows;
+  int channels;                         /* 1 ... 8192 */
+  long long gate_rows;
+  int rms;                              /* 0: LayerNorm, 1: RMSNorm */
+  float residual_scale, eps;
+} fdx_resnorm_desc;
+int fdx_resnorm_forward(fdx_handle h, const fdx_resnorm_desc* d, const void* x, const void* block, const void* gate, const void* post_w,
+                        const void* post_b, const void* pre_w, const void* pre_b, void* out_h, void* out_y, float* stats, fdx_stream s);
+/* grad_h / grad_y may be NULL (zero).  dblock may be dx itself where the two are equal (no gate, no post norm, residual_scale 1).  Sums over rows are
+ * taken in a fixed order.  Gradients of weights and biases have param_dtype, dgate gate_dtype; NULL weights have NULL gradients. */
+int fdx_resnorm_backward_workspace(const fdx_resnorm_desc* d, size_t* bytes);
+int fdx_resnorm_backward(fdx_handle h, const fdx_resnorm_desc* d, const void* grad_h, const void* grad_y, const void* x, const void* block,
+                         const void* gate, const void* post_w, const void* post_b, const void* pre_w, const void* pre_b, const float* stats,
+                         void* dx, void* dblock, void* dgate, void* dpost_w, void* dpost_b, void* dpre_w, void* dpre_b, void* workspace,
+                         size_t bytes, fdx_stream s);
+
+/* Activations kept in 8 bits for the backward pass.  x dev [rows][channels]; codes dev [rows][channels]; exps dev [rows][ceil(channels / 32)]: a group of
+ * 32 channels shares 2^(e - 127), e >= 1 the smallest with max|x| <= 127 * 2^(e - 127); code = x / 2^(e - 127), nearest even
+ * (at the largest exponent, 249, at most 63: no finite x reads back as infinity).  A group with an infinity or NaN has e = 255 and reads back as NaN.
+ * dtype: that of x (fdx_unpack8: of the values written; fp16 ends at 65504). */
+int fdx_pack8(fdx_handle h, int dtype, const void* x, long long rows, int channels, int8_t* codes, uint8_t* exps, fdx_stream s);
+int fdx_unpack8(fdx_handle h, int dtype, const int8_t* codes, const uint8_t* exps, long long rows, int channels, void* x, fdx_stream s);
+/* y = gelu(x) (erf form) with x kept in 8 bits; dx = dy gelu'(x8).  dx may be dy. */
+int fdx_gelu8_forward(fdx_handle h, int dtype, const void* x, long long rows, int channels, void* y, int8_t* codes, uint8_t* exps, fdx_stream s);
+int fdx_gelu8_backward(fdx_handle h, int dtype, const void* dy, const int8_t* codes, const uint8_t* exps, long long rows, int channels, void* dx,
+                       fdx_stream s);
+/* dw [out_features][in_features] = dy^T x8, db [out_features] = the sum of dy over the rows (NULL: not wanted); dy dev [rows][out_features] of dtype,
+ * dw / db of grad_dtype.  Every product is exact (x8 is a bf16 number, dy is split into bf16 numbers), sums are fp32 in a fixed order; where dy holds an
+ * infinity the sums it enters are NaN in fp32 and fp16. */
+int fdx_linear8_weight_grad_workspace(int dtype, long long rows, int out_features, int in_features, size_t* bytes);
+int fdx_linear8_weight_grad(fdx_handle h, int dtype, const void* dy, const int8_t* codes, const uint8_t* exps, long long rows, int out_features,
+                            int in_features, int grad_dtype, void* dw, void* db, void* workspace, size_t bytes, fdx_stream s);
+
 /* ------------------------------------------------------------------------------------------------
  * Kernel-level test / profiling hooks (used by tests/ and bench.py only)
  * ---------------------------------------------------------------------------------------------- */
