@@ -7,8 +7,8 @@
 //
 // Bound by memory: forward reads x, block, writes h, y; backward reads x, block, grad_h, grad_y and writes dx, dblock.  n, h and both normalised
 // tensors are computed again from x and block in fp32 (reading h, y instead of x would cost the same bytes and add their rounding); the forward
-// leaves mean and 1 / deviation of both norms (16 bytes a row).  One wave holds a row in registers up to 2048 channels (backward 1024), 4 or 8
-// waves above; means are taken before the squares are summed (two passes over registers).  The sums over rows run per thread in row order,
+// leaves mean and 1 / deviation of both norms (16 bytes a row).  One wave holds a row of up to 512 channels in registers, 2, 4 or 8 waves
+// a longer one; means are taken before the squares are summed (two passes over registers).  The sums over rows run per thread in row order,
 // then over the waves of a workgroup in LDS, then over the workgroups in a second launch, always in the same order.
 #include "tileops.hip.h"
 
@@ -35,15 +35,17 @@ struct NormArgs {
 
 // -------------------------------------------------------------------------------------------------------------- pieces of a row
 // A thread's IT pieces of VEC channels: channel (i * threads + t) * VEC + j.
-template <typename T, int VEC> __device__ inline void ld(const T* p, float* v) {
-  if constexpr (VEC == 1) v[0] = (float)*p;
-  else {
-    typedef T vt __attribute__((ext_vector_type(VEC)));
-    const vt r = *reinterpret_cast<const vt*>(p);
-#pragma unroll
-    for (int j = 0; j < VEC; ++j) v[j] = (float)r[j];
-  }
-}
+template <typename T, int VEC> struct Piece {   // as loaded
+  typedef T vt __attribute__((ext_vector_type(VEC)));
+  vt v;
+  __device__ inline void load(const T* p) { v = *reinterpret_cast<const vt*>(p); }
+  __device__ inline float at(int j) const { return (float)v[j]; }
+};
+template <typename T> struct Piece<T, 1> {
+  T v;
+  __device__ inline void load(const T* p) { v = *p; }
+  __device__ inline float at(int) const { return (float)v; }
+};
 template <typename T, int VEC> __device__ inline void st(T* p, const float* v) {
   if constexpr (VEC == 1) *p = (T)v[0];
   else {
@@ -55,10 +57,21 @@ template <typename T, int VEC> __device__ inline void st(T* p, const float* v) {
   }
 }
 template <typename T, int VEC> __device__ inline void ldp(const void* p, int dt, long i, float* v) {   // parameter: T or fp32
-  if (DtOf<T>::v == DT_F32 || dt != DT_F32) ld<T, VEC>(static_cast<const T*>(p) + i, v);
-  else {
+  if (DtOf<T>::v == DT_F32 || dt != DT_F32) {
+    Piece<T, VEC> r;
+    r.load(static_cast<const T*>(p) + i);
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) v[j] = r.at(j);
+  } else {
 #pragma unroll
     for (int j = 0; j < VEC; ++j) v[j] = static_cast<const float*>(p)[i + j];
+  }
+}
+template <typename T, int VEC> __device__ inline void stp(void* p, int dt, long i, const float* v) {
+  if (DtOf<T>::v == DT_F32 || dt != DT_F32) st<T, VEC>(static_cast<T*>(p) + i, v);
+  else {
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) static_cast<float*>(p)[i + j] = v[j];
   }
 }
 
@@ -75,97 +88,118 @@ __device__ inline float wave_sum(float x) {
   x = dpp_add<0x143, 0xc>(x);
   return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, x), 63));
 }
-// over the NW waves of a unit (NW > 1: the whole workgroup); `buf` alternates between two blocks of 2 * NW floats
-template <int NW> __device__ inline void unit_sum(float& a, float& b, float* buf, int& turn) {
-  a = wave_sum(a);
-  b = wave_sum(b);
-  if constexpr (NW > 1) {
-    float* p = buf + turn * 2 * NW;
-    turn ^= 1;
-    const int w = threadIdx.x >> 6;
-    if ((threadIdx.x & 63) == 0) { p[w] = a; p[NW + w] = b; }
-    __syncthreads();
-    a = b = 0.f;
-#pragma unroll
-    for (int i = 0; i < NW; ++i) { a += p[i]; b += p[NW + i]; }
-  }
-}
 
-template <typename T, int VEC, int IT, int NW> struct Row {
-  static constexpr int NT = 64 * NW, E = VEC * IT;
-  static constexpr int kThreads = NW > 4 ? 64 * NW : 256, kUnits = kThreads / NT;
+template <typename T, int VEC_, int IT_, int NW_> struct Row {
+  static constexpr int VEC = VEC_, IT = IT_, NW = NW_, NT = 64 * NW, E = VEC * IT;
+  static constexpr int kThreads = NW > 1 ? NT : 256, kUnits = kThreads / NT;   // NW > 1: one row at a time per workgroup
+  typedef Piece<T, VEC> Raw[IT];
   static __device__ inline int col(int i) { return (i * NT + (int)threadIdx.x % NT) * VEC; }
   template <typename F> static __device__ inline void each(int C, F&& f) {
 #pragma unroll
     for (int i = 0; i < IT; ++i)
       if (col(i) < C) f(col(i), i * VEC);
   }
+  static __device__ inline void load(Raw& r, const void* p, long o, int C) {
+#pragma unroll
+    for (int i = 0; i < IT; ++i)
+      if (col(i) < C) r[i].load(static_cast<const T*>(p) + o + col(i));
+  }
+  static __device__ inline void widen(const Raw& r, float (&v)[E]) {
+#pragma unroll
+    for (int i = 0; i < IT; ++i)
+#pragma unroll
+      for (int j = 0; j < VEC; ++j) v[i * VEC + j] = r[i].at(j);
+  }
+  static __device__ inline void param(const void* p, int dt, int C, float other, float (&v)[E]) {   // `other` where there is none
+#pragma unroll
+    for (int e = 0; e < E; ++e) v[e] = other;
+    if (p) each(C, [&](int c, int e) { ldp<T, VEC>(p, dt, c, v + e); });
+  }
+  // sums over the row's waves; `buf` alternates between two blocks of 2 * NW floats
+  static __device__ inline void sum(float& a, float& b, float* buf, int& turn) {
+    a = wave_sum(a);
+    b = wave_sum(b);
+    if constexpr (NW > 1) {
+      float* p = buf + turn * 2 * NW;
+      turn ^= 1;
+      const int w = threadIdx.x >> 6;
+      if ((threadIdx.x & 63) == 0) { p[w] = a; p[NW + w] = b; }
+      __syncthreads();
+      a = b = 0.f;
+#pragma unroll
+      for (int i = 0; i < NW; ++i) { a += p[i]; b += p[NW + i]; }
+    }
+  }
+  // mean (RMSNorm: 0) and 1 / sqrt(variance + eps)
+  static __device__ inline void stats(const float (&v)[E], const NormArgs& a, float* buf, int& turn, float& mean, float& rstd) {
+    float s = 0.f, none = 0.f;
+    mean = 0.f;
+    if (!a.rms) {
+      each(a.C, [&](int, int e) {
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) s += v[e + j];
+      });
+      sum(s, none, buf, turn);
+      mean = s * a.inv_c;
+    }
+    float q = 0.f;
+    each(a.C, [&](int, int e) {
+#pragma unroll
+      for (int j = 0; j < VEC; ++j) { const float d = v[e + j] - mean; q = __builtin_fmaf(d, d, q); }
+    });
+    none = 0.f;
+    sum(q, none, buf, turn);
+    rstd = 1.f / sqrtf(q * a.inv_c + a.eps);
+  }
 };
 
-// mean (RMSNorm: 0) and 1 / sqrt(variance + eps) of a row
-template <typename R, int VEC, int NW> __device__ inline void stats_of(const float* v, const NormArgs& a, float* buf, int& turn, float& mean, float& rstd) {
-  float s = 0.f, none = 0.f;
-  mean = 0.f;
-  if (!a.rms) {
-    R::each(a.C, [&](int, int e) {
-#pragma unroll
-      for (int j = 0; j < VEC; ++j) s += v[e + j];
-    });
-    unit_sum<NW>(s, none, buf, turn);
-    mean = s * a.inv_c;
-  }
-  float q = 0.f;
-  R::each(a.C, [&](int, int e) {
-#pragma unroll
-    for (int j = 0; j < VEC; ++j) { const float d = v[e + j] - mean; q = __builtin_fmaf(d, d, q); }
-  });
-  none = 0.f;
-  unit_sum<NW>(q, none, buf, turn);
-  rstd = 1.f / sqrtf(q * a.inv_c + a.eps);
-}
-
-// h (holding x) <- a x + g n
-template <typename R, int VEC> __device__ inline void gate_and_add(const NormArgs& a, const float (&g)[R::E], const float (&n)[R::E], float (&h)[R::E]) {
-  R::each(a.C, [&](int, int e) {
-#pragma unroll
-    for (int j = 0; j < VEC; ++j) h[e + j] = __builtin_fmaf(a.a, h[e + j], a.gate ? g[e + j] * n[e + j] : n[e + j]);
-  });
-}
-template <typename T, typename R, int VEC>
-__device__ inline void affine(const NormArgs& a, const void* w, const void* b, float mean, float rstd, float* v) {
-  R::each(a.C, [&](int c, int e) {
-    float wv[VEC], bv[VEC];
-    ldp<T, VEC>(w, a.pdt, c, wv);
-    if (b) ldp<T, VEC>(b, a.pdt, c, bv);
-#pragma unroll
-    for (int j = 0; j < VEC; ++j) v[e + j] = __builtin_fmaf((v[e + j] - mean) * rstd, wv[j], b ? bv[j] : 0.f);
-  });
-}
-
+// Rows are taken in turn by a fixed number of units, the next row's loads issued before this one's sums: with two workgroups on a CU and a barrier per
+// sum the loads' latency is what costs otherwise.  The norms' parameters stay in registers.
 template <typename T, int VEC, int IT, int NW>
 __global__ __launch_bounds__((Row<T, VEC, IT, NW>::kThreads)) void k_resnorm_fwd(NormArgs a) {
   typedef Row<T, VEC, IT, NW> R;
+  constexpr int E = R::E;
   __shared__ float buf[NW > 1 ? 4 * NW : 1];
   int turn = 0;
-  const int unit = threadIdx.x / R::NT;
-  for (long row = (long)blockIdx.x * R::kUnits + unit; row < a.N; row += (long)gridDim.x * R::kUnits) {
+  float pw[E], pb[E], nw[E], nb[E];
+  R::param(a.post_w, a.pdt, a.C, 1.f, pw);
+  R::param(a.post_b, a.pdt, a.C, 0.f, pb);
+  R::param(a.pre_w, a.pdt, a.C, 1.f, nw);
+  R::param(a.pre_b, a.pdt, a.C, 0.f, nb);
+  const long step = (long)gridDim.x * R::kUnits;
+  long row = (long)blockIdx.x * R::kUnits + threadIdx.x / R::NT;
+  typename R::Raw rx, rb;
+  if (row < a.N) {
+    R::load(rx, a.x, row * a.C, a.C);
+    R::load(rb, a.block, row * a.C, a.C);
+  }
+  for (; row < a.N; row += step) {
     const long o = row * a.C;
-    float x[R::E], n[R::E], g[R::E];
-    R::each(a.C, [&](int c, int e) {
-      ld<T, VEC>(static_cast<const T*>(a.x) + o + c, x + e);
-      ld<T, VEC>(static_cast<const T*>(a.block) + o + c, n + e);
-      if (a.gate) ldp<T, VEC>(a.gate, a.gdt, row / a.gate_rows * a.C + c, g + e);
-    });
+    float x[E], n[E];
+    R::widen(rx, x);
+    R::widen(rb, n);
+    float g[E];
+    if (a.gate) {
+      const long at = a.gate_rows == 1 ? o : a.gate_rows == a.N ? 0 : row / a.gate_rows * a.C;
+      R::each(a.C, [&](int c, int e) { ldp<T, VEC>(a.gate, a.gdt, at + c, g + e); });
+    }
+    if (row + step < a.N) {
+      R::load(rx, a.x, (row + step) * a.C, a.C);
+      R::load(rb, a.block, (row + step) * a.C, a.C);
+    }
     float m0 = 0.f, r0 = 0.f, m1 = 0.f, r1 = 0.f;
     if (a.has_post) {
-      stats_of<R, VEC, NW>(n, a, buf, turn, m0, r0);
-      affine<T, R, VEC>(a, a.post_w, a.post_b, m0, r0, n);
+      R::stats(n, a, buf, turn, m0, r0);
+#pragma unroll
+      for (int e = 0; e < E; ++e) n[e] = __builtin_fmaf((n[e] - m0) * r0, pw[e], pb[e]);
     }
-    gate_and_add<R, VEC>(a, g, n, x);
+#pragma unroll
+    for (int e = 0; e < E; ++e) x[e] = __builtin_fmaf(a.a, x[e], a.gate ? g[e] * n[e] : n[e]);
     R::each(a.C, [&](int c, int e) { st<T, VEC>(static_cast<T*>(a.h) + o + c, x + e); });
     if (a.has_pre) {
-      stats_of<R, VEC, NW>(x, a, buf, turn, m1, r1);
-      affine<T, R, VEC>(a, a.pre_w, a.pre_b, m1, r1, x);
+      R::stats(x, a, buf, turn, m1, r1);
+#pragma unroll
+      for (int e = 0; e < E; ++e) x[e] = __builtin_fmaf((x[e] - m1) * r1, nw[e], nb[e]);
       R::each(a.C, [&](int c, int e) { st<T, VEC>(static_cast<T*>(a.y) + o + c, x + e); });
     }
     if (a.stats && threadIdx.x % R::NT == 0) *reinterpret_cast<f32x4*>(a.stats + 4 * row) = f32x4{m0, r0, m1, r1};
@@ -194,56 +228,63 @@ __global__ __launch_bounds__((Row<T, VEC, IT, NW>::kThreads)) void k_resnorm_bwd
     end = grp * a.rows_per_group + min((cut + 1) * per, a.rows_per_group);
     step = R::kUnits;
   }
-  float sum[5][E];
+  float sum[5][E], pw[E], pb[E], nw[E];
 #pragma unroll
   for (int s = 0; s < 5; ++s)
 #pragma unroll
     for (int e = 0; e < E; ++e) sum[s][e] = 0.f;
-
+  R::param(a.post_w, a.pdt, a.C, 1.f, pw);
+  R::param(a.post_b, a.pdt, a.C, 0.f, pb);
+  R::param(a.pre_w, a.pdt, a.C, 1.f, nw);
+  typename R::Raw rx, rb, rh, ry;
+  f32x4 ms = {0, 0, 0, 0};
+  auto fetch = [&](long row) {
+    const long o = row * a.C;
+    if (a.gy) { R::load(rx, a.x, o, a.C); R::load(ry, a.gy, o, a.C); }
+    R::load(rb, a.block, o, a.C);
+    if (a.gh) R::load(rh, a.gh, o, a.C);
+    ms = *reinterpret_cast<const f32x4*>(a.stats + 4 * row);
+  };
+  if (r < end) fetch(r);
   // units of one wave may run out of rows at different times: none of them waits for another one in the loop (NW > 1: one unit per workgroup)
   for (; r < end; r += step) {
     const long o = r * a.C;
-    float h[E], n[E], g[E], gh[E], gy[E];
-    R::each(a.C, [&](int c, int e) {
-      if (a.has_pre) ld<T, VEC>(static_cast<const T*>(a.x) + o + c, h + e);
-      ld<T, VEC>(static_cast<const T*>(a.block) + o + c, n + e);
-      if (a.gate) ldp<T, VEC>(a.gate, a.gdt, r / a.gate_rows * a.C + c, g + e);
-      if (a.gh) ld<T, VEC>(static_cast<const T*>(a.gh) + o + c, gh + e);
-      if (a.gy) ld<T, VEC>(static_cast<const T*>(a.gy) + o + c, gy + e);
-    });
-    const f32x4 ms = *reinterpret_cast<const f32x4*>(a.stats + 4 * r);
     const float m0 = ms[0], r0 = ms[1], m1 = ms[2], r1 = ms[3];
-    if (a.has_post) affine<T, R, VEC>(a, a.post_w, a.post_b, m0, r0, n);
-    float dh[E];
+    float h[E], bhat[E], gy[E], dh[E], g[E];
+    R::widen(rb, bhat);
+#pragma unroll
+    for (int e = 0; e < E; ++e) dh[e] = 0.f;
+    if (a.gh) R::widen(rh, dh);
+    if (a.gy) { R::widen(rx, h); R::widen(ry, gy); }
+    if (a.gate) {
+      const long at = a.gate_rows == 1 ? o : a.gate_rows == a.N ? 0 : r / a.gate_rows * a.C;
+      R::each(a.C, [&](int c, int e) { ldp<T, VEC>(a.gate, a.gdt, at + c, g + e); });
+    }
+    if (r + step < end) fetch(r + step);
+    if (a.has_post) {
+#pragma unroll
+      for (int e = 0; e < E; ++e) bhat[e] = (bhat[e] - m0) * r0;
+    }
+    auto n = [&](int e) { return a.has_post ? __builtin_fmaf(bhat[e], pw[e], pb[e]) : bhat[e]; };
     if (a.gy) {
-      gate_and_add<R, VEC>(a, g, n, h);
       float s1 = 0.f, s2 = 0.f;
-      R::each(a.C, [&](int c, int e) {
-        float w[VEC];
-        ldp<T, VEC>(a.pre_w, a.pdt, c, w);
+      R::each(a.C, [&](int, int e0) {
 #pragma unroll
         for (int j = 0; j < VEC; ++j) {
-          const float hat = (h[e + j] - m1) * r1;
-          sum[1][e + j] = __builtin_fmaf(gy[e + j], hat, sum[1][e + j]);
-          sum[2][e + j] += gy[e + j];
-          gy[e + j] *= w[j];
-          h[e + j] = hat;
-          s1 += gy[e + j];
-          s2 = __builtin_fmaf(gy[e + j], hat, s2);
+          const int e = e0 + j;
+          h[e] = (__builtin_fmaf(a.a, h[e], a.gate ? g[e] * n(e) : n(e)) - m1) * r1;   // normalised h
+          sum[1][e] = __builtin_fmaf(gy[e], h[e], sum[1][e]);
+          sum[2][e] += gy[e];
+          gy[e] *= nw[e];
+          s1 += gy[e];
+          s2 = __builtin_fmaf(gy[e], h[e], s2);
         }
       });
-      unit_sum<NW>(s1, s2, buf, turn);
+      R::sum(s1, s2, buf, turn);
       s1 = a.rms ? 0.f : s1 * a.inv_c;
       s2 *= a.inv_c;
-      R::each(a.C, [&](int, int e) {
 #pragma unroll
-        for (int j = 0; j < VEC; ++j) dh[e + j] = __builtin_fmaf(r1, gy[e + j] - s1 - h[e + j] * s2, a.gh ? gh[e + j] : 0.f);
-      });
-    } else {
-      R::each(a.C, [&](int, int e) {
-#pragma unroll
-        for (int j = 0; j < VEC; ++j) dh[e + j] = a.gh ? gh[e + j] : 0.f;
-      });
+      for (int e = 0; e < E; ++e) dh[e] = __builtin_fmaf(r1, gy[e] - s1 - h[e] * s2, dh[e]);
     }
     R::each(a.C, [&](int c, int e) {
       float v[VEC];
@@ -256,50 +297,38 @@ __global__ __launch_bounds__((Row<T, VEC, IT, NW>::kThreads)) void k_resnorm_bwd
         float v[VEC];
 #pragma unroll
         for (int j = 0; j < VEC; ++j) {
-          v[j] = dh[e + j] * n[e + j];
+          v[j] = dh[e + j] * n(e + j);
           sum[0][e + j] += v[j];
           dh[e + j] *= g[e + j];   // dn
         }
-        if (a.gate_rows == 1) {
-          if (a.gdt == DT_F32) st<float, VEC>(static_cast<float*>(a.dgate) + o + c, v);
-          else st<T, VEC>(static_cast<T*>(a.dgate) + o + c, v);
-        }
+        if (a.gate_rows == 1) stp<T, VEC>(a.dgate, a.gdt, o + c, v);
       });
       if (a.flush && (r + 1) % a.rows_per_group == 0) {
         R::each(a.C, [&](int c, int e) {
-          const long at = r / a.rows_per_group * a.C + c;
-          if (a.gdt == DT_F32) st<float, VEC>(static_cast<float*>(a.dgate) + at, sum[0] + e);
-          else st<T, VEC>(static_cast<T*>(a.dgate) + at, sum[0] + e);
+          stp<T, VEC>(a.dgate, a.gdt, r / a.rows_per_group * a.C + c, sum[0] + e);
 #pragma unroll
           for (int j = 0; j < VEC; ++j) sum[0][e + j] = 0.f;
         });
       }
     }
     if (a.has_post) {
-      // block again (its registers became n)
       float s1 = 0.f, s2 = 0.f;
-      R::each(a.C, [&](int c, int e) {
-        float w[VEC], b[VEC];
-        ldp<T, VEC>(a.post_w, a.pdt, c, w);
-        ld<T, VEC>(static_cast<const T*>(a.block) + o + c, b);
+      R::each(a.C, [&](int, int e0) {
 #pragma unroll
         for (int j = 0; j < VEC; ++j) {
-          const float hat = (b[j] - m0) * r0;
-          sum[3][e + j] = __builtin_fmaf(dh[e + j], hat, sum[3][e + j]);
-          sum[4][e + j] += dh[e + j];
-          dh[e + j] *= w[j];
-          n[e + j] = hat;
-          s1 += dh[e + j];
-          s2 = __builtin_fmaf(dh[e + j], hat, s2);
+          const int e = e0 + j;
+          sum[3][e] = __builtin_fmaf(dh[e], bhat[e], sum[3][e]);
+          sum[4][e] += dh[e];
+          dh[e] *= pw[e];
+          s1 += dh[e];
+          s2 = __builtin_fmaf(dh[e], bhat[e], s2);
         }
       });
-      unit_sum<NW>(s1, s2, buf, turn);
+      R::sum(s1, s2, buf, turn);
       s1 = a.rms ? 0.f : s1 * a.inv_c;
       s2 *= a.inv_c;
-      R::each(a.C, [&](int, int e) {
 #pragma unroll
-        for (int j = 0; j < VEC; ++j) dh[e + j] = r0 * (dh[e + j] - s1 - n[e + j] * s2);
-      });
+      for (int e = 0; e < E; ++e) dh[e] = r0 * (dh[e] - s1 - bhat[e] * s2);
     }
     if (!a.same_dx) R::each(a.C, [&](int c, int e) { st<T, VEC>(static_cast<T*>(a.dblock) + o + c, dh + e); });
   }
@@ -339,20 +368,34 @@ struct NormJoin {
   int dt[5], C, wgs, gate_cuts;   // gate_cuts: workgroups per gate row (slot 0 with more than one row), 0: as the others
   int n_out, slot[5];
 };
-template <typename T> __global__ __launch_bounds__(256) void k_resnorm_join(NormJoin a) {
-  __shared__ float red[4][64];
-  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, c = blockIdx.x * 64 + lane;
+// A workgroup: 32 channels, 32 threads each; a thread sums every 32nd partial row, eight loads in flight.
+template <typename T> __global__ __launch_bounds__(1024) void k_resnorm_join(NormJoin a) {
+  __shared__ float red[32][32];
+  const int lane = threadIdx.x & 31, w = threadIdx.x >> 5, c = blockIdx.x * 32 + lane;
   int s, first = 0, last = a.wgs, k;
   long row = 0;
   if ((int)blockIdx.y < a.n_out) { k = blockIdx.y; s = a.slot[k]; }
   else { s = 0; k = a.n_out; row = (int)blockIdx.y - a.n_out; first = (int)row * a.gate_cuts; last = first + a.gate_cuts; }
   float v = 0.f;
-  if (c < a.C)
-    for (int i = first + w; i < last; i += 4) v += a.part[((long)i * 5 + s) * a.C + c];
+  if (c < a.C) {
+    const float* p = a.part + (long)s * a.C + c;
+    const long pitch = 5L * a.C;
+    int i = first + w;
+    for (; i + 7 * 32 < last; i += 8 * 32) {
+      float t[8];
+#pragma unroll
+      for (int q = 0; q < 8; ++q) t[q] = p[(i + q * 32) * pitch];
+#pragma unroll
+      for (int q = 0; q < 8; ++q) v += t[q];
+    }
+    for (; i < last; i += 32) v += p[i * pitch];
+  }
   red[w][lane] = v;
   __syncthreads();
   if (w == 0 && c < a.C) {
-    v = red[0][lane] + red[1][lane] + red[2][lane] + red[3][lane];
+    v = 0.f;
+#pragma unroll
+    for (int i = 0; i < 32; ++i) v += red[i][lane];
     if (a.dt[k] == DT_F32) static_cast<float*>(a.out[k])[row * a.C + c] = v;
     else static_cast<T*>(a.out[k])[row * a.C + c] = (T)v;
   }
@@ -387,15 +430,12 @@ Cut cut_of(const fdx_resnorm_desc* d, int units) {
   return c;
 }
 
-struct Shape { int vec, it, nw; };   // pieces of a row per thread and waves per row
-Shape shape_of(const fdx_resnorm_desc* d, bool vec, bool bwd) {
+// 8 channels a thread (16 above 4096 channels) and as many waves as that takes: the backward pass holds five sums and five values per channel, and with 8 of
+// them two to three workgroups of four waves fit on a CU.
+struct Shape { int vec, it, nw; };
+Shape shape_of(const fdx_resnorm_desc* d, bool vec) {
   const int v = !vec ? 1 : d->dtype == DT_F32 ? 4 : 8, C = d->channels;
-  const int per1 = bwd ? 16 : 32;   // channels a thread may hold with one wave per row
-  if (C <= 64 * 8) return {v, 8 / v, 1};
-  if (C <= 64 * 16) return {v, 16 / v, 1};
-  if (C <= 64 * per1) return {v, 32 / v, 1};
-  if (C <= 256 * 16) return {v, 16 / v, 4};
-  return {v, 16 / v, 8};
+  return C <= 4096 ? Shape{v, 8 / v, C <= 512 ? 1 : C <= 1024 ? 2 : C <= 2048 ? 4 : 8} : Shape{v, 16 / v, 8};
 }
 
 template <typename T, int VEC, bool BWD, int IT, int NW> hipError_t run(const NormArgs& a, unsigned grid, hipStream_t s) {
@@ -403,13 +443,12 @@ template <typename T, int VEC, bool BWD, int IT, int NW> hipError_t run(const No
   else return launch(k_resnorm_fwd<T, VEC, IT, NW>, grid, Row<T, VEC, IT, NW>::kThreads, a, s);
 }
 template <typename T, int VEC, bool BWD> hipError_t run(const NormArgs& a, Shape sh, unsigned grid, hipStream_t s) {
-  constexpr int A = 8 / VEC, B = 16 / VEC, D = 32 / VEC;
-  if (sh.nw == 1 && sh.it == A) return run<T, VEC, BWD, A, 1>(a, grid, s);
-  if (sh.nw == 1 && sh.it == B) return run<T, VEC, BWD, B, 1>(a, grid, s);
-  if constexpr (!BWD)
-    if (sh.nw == 1) return run<T, VEC, BWD, D, 1>(a, grid, s);
-  if (sh.nw == 4) return run<T, VEC, BWD, B, 4>(a, grid, s);
-  return run<T, VEC, BWD, B, 8>(a, grid, s);
+  constexpr int A = 8 / VEC, B = 16 / VEC;
+  if (sh.it == B) return run<T, VEC, BWD, B, 8>(a, grid, s);
+  if (sh.nw == 1) return run<T, VEC, BWD, A, 1>(a, grid, s);
+  if (sh.nw == 2) return run<T, VEC, BWD, A, 2>(a, grid, s);
+  if (sh.nw == 4) return run<T, VEC, BWD, A, 4>(a, grid, s);
+  return run<T, VEC, BWD, A, 8>(a, grid, s);
 }
 template <bool BWD> hipError_t by_type(const fdx_resnorm_desc* d, const NormArgs& a, Shape sh, unsigned grid, hipStream_t s) {
   const bool one = sh.vec == 1;
@@ -445,21 +484,18 @@ extern "C" int fdx_resnorm_forward(fdx_handle h, const fdx_resnorm_desc* d, cons
   NormArgs a = args_of(d);
   a.x = x; a.block = block; a.gate = gate; a.post_w = post_w; a.post_b = post_b; a.pre_w = pre_w; a.pre_b = pre_b;
   a.h = out_h; a.y = out_y; a.stats = stats; a.has_post = post_w != nullptr; a.has_pre = pre_w != nullptr;
-  const Shape sh = shape_of(d, vec_ok(d, {x, block, gate, post_w, post_b, pre_w, pre_b, out_h, out_y}), false);
-  const long units = units_of(sh), grid = std::min<long>((d->rows + units - 1) / units, 1L << 20);
+  const Shape sh = shape_of(d, vec_ok(d, {x, block, gate, post_w, post_b, pre_w, pre_b, out_h, out_y}));
+  const long units = units_of(sh), grid = std::min<long>((d->rows + units - 1) / units, 1024 * 4 / std::max(4, sh.nw));
   DeviceScope dev(h->device);
   FDX_HIP(h, dev.err);
   FDX_HIP(h, by_type<false>(d, a, sh, (unsigned)grid, as_stream(st)));
   return FDX_OK;
 }
 
-// (the larger of the two shapes the launch may take: the workspace does not depend on the tensors' alignment)
 extern "C" int fdx_resnorm_backward_workspace(const fdx_resnorm_desc* d, size_t* bytes) {
   if (const char* why = check(d)) return fail(nullptr, FDX_E_ARG, "fdx_resnorm_backward_workspace: %s", why);
   if (!bytes) return fail(nullptr, FDX_E_ARG, "fdx_resnorm_backward_workspace: null size pointer");
-  size_t n = 0;
-  for (bool vec : {false, true}) n = std::max<size_t>(n, cut_of(d, units_of(shape_of(d, vec, true))).wgs);
-  *bytes = n * 5 * d->channels * sizeof(float);
+  *bytes = (size_t)cut_of(d, units_of(shape_of(d, true))).wgs * 5 * d->channels * sizeof(float);
   return FDX_OK;
 }
 
@@ -481,7 +517,7 @@ extern "C" int fdx_resnorm_backward(fdx_handle h, const fdx_resnorm_desc* d, con
   a.same_dx = dblock == dx;
   if (a.same_dx && (post_w || gate || d->residual_scale != 1.f))
     return fail(h, FDX_E_ARG, "fdx_resnorm_backward: dblock may be dx only where they are equal (no gate, no post norm, residual_scale 1)");
-  const Shape sh = shape_of(d, vec_ok(d, {x, block, gate, post_w, post_b, pre_w, pre_b, grad_h, grad_y, dx, dblock, dgate}), true);
+  const Shape sh = shape_of(d, vec_ok(d, {x, block, gate, post_w, post_b, pre_w, pre_b, grad_h, grad_y, dx, dblock, dgate}));
   const Cut c = cut_of(d, units_of(sh));
   const size_t need = (size_t)c.wgs * 5 * d->channels * sizeof(float);
   if (bytes < need || !workspace || (reinterpret_cast<uintptr_t>(workspace) & 15))
@@ -506,11 +542,11 @@ extern "C" int fdx_resnorm_backward(fdx_handle h, const fdx_resnorm_desc* d, con
   FDX_HIP(h, dev.err);
   FDX_HIP(h, by_type<true>(d, a, sh, (unsigned)c.wgs, as_stream(st)));
   if (j.n_out + gate_out > 0) {
-    const dim3 grid((d->channels + 63) / 64, j.n_out + gate_out);
+    const dim3 grid((d->channels + 31) / 32, j.n_out + gate_out);
     void* argv[] = {&j};
     const void* k = d->dtype == DT_BF16 ? reinterpret_cast<const void*>(k_resnorm_join<bf16_t>)
                     : d->dtype == DT_F16 ? reinterpret_cast<const void*>(k_resnorm_join<f16_t>) : reinterpret_cast<const void*>(k_resnorm_join<float>);
-    FDX_HIP(h, hipLaunchKernel(k, grid, dim3(256), argv, 0, as_stream(st)));
+    FDX_HIP(h, hipLaunchKernel(k, grid, dim3(1024), argv, 0, as_stream(st)));
   }
   return FDX_OK;
 }

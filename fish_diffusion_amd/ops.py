@@ -60,55 +60,70 @@ def _apply(fn, *args):
 
 
 def _dtype(t: torch.Tensor, what: str) -> int:
-    if t.dtype not in _lib.DTYPES:
+    dt = _lib.DTYPES.get(t.dtype)
+    if dt is None:
         raise TypeError(f"{what}: {t.dtype} is not one of float32, bfloat16, float16")
-    return _lib.DTYPES[t.dtype]
+    return dt
 
 
 def _same(ref: torch.Tensor, what: str, **tensors):
+    device, dtype = ref.device, ref.dtype
     for name, t in tensors.items():
         if t is None:
             continue
-        _lib.require_gpu(t, f"{what} {name}")
-        if t.device != ref.device:
-            raise ValueError(f"{what}: {name} is on {t.device}, expected {ref.device}")
-        if t.dtype != ref.dtype:
-            raise ValueError(f"{what}: {name} is {t.dtype}, expected {ref.dtype}")
+        if t.device != device:
+            _lib.require_gpu(t, f"{what} {name}")
+            raise ValueError(f"{what}: {name} is on {t.device}, expected {device}")
+        if t.dtype != dtype:
+            raise ValueError(f"{what}: {name} is {t.dtype}, expected {dtype}")
+
+
+_handles = {}
 
 
 def _handle(device: torch.device) -> _lib.Handle:
-    with torch.cuda.device(device):   # creating a handle makes its device current
-        return _lib.Handle.shared(device)
+    h = _handles.get(device.index)
+    if h is None:
+        with torch.cuda.device(device):   # creating a handle makes its device current
+            h = _handles[device.index] = _lib.Handle.shared(device)
+    return h
 
 
-def _aligned(t: torch.Tensor) -> torch.Tensor:
-    """The tensor itself where the kernels can read it in 16-byte pieces along its last dimension, else a contiguous copy."""
-    es = t.element_size()
-    if t.numel() == 0:
-        return t
-    ok = t.data_ptr() % 16 == 0 and (t.shape[-1] == 1 or t.stride(-1) == 1)
-    ok = ok and all(n == 1 or s * es % 16 == 0 for n, s in zip(t.shape[:-1], t.stride()[:-1]))
-    return t if ok else t.clone(memory_format=torch.contiguous_format)
+def _stream(h: _lib.Handle):
+    return torch._C._cuda_getCurrentRawStream(h.device.index)   # torch.cuda.current_stream(device).cuda_stream without its objects: 2 us less a call
 
 
-def _bht(t: Optional[torch.Tensor]):
-    if t is None or t.numel() == 0:
-        return _lib.Bht(None, 0, 0, 0)
-    s = [0 if n == 1 else st for n, st in zip(t.shape[:3], t.stride()[:3])]
-    return _lib.Bht(t.data_ptr(), *s)
+def _copy(t: torch.Tensor) -> torch.Tensor:
+    return t.detach().clone(memory_format=torch.contiguous_format)
+
+
+def _p(t: Optional[torch.Tensor]):
+    return None if t is None else t.data_ptr()
+
+
+def _arg(t: torch.Tensor, vec: int):
+    """(tensor, its description for the C call); a contiguous copy where the kernels cannot read it in 16-byte pieces of `vec` elements."""
+    at, (b, h, n, _), (sb, sh, sn, sd) = t.data_ptr(), t.shape, t.stride()
+    sb, sh, sn = (sb if b > 1 else 0), (sh if h > 1 else 0), (sn if n > 1 else 0)
+    if (at & 15 or sd != 1 or (sb | sh | sn) & (vec - 1)) and t.numel():
+        return _arg(_copy(t), vec)
+    return t, _lib.Bht(at or None, sb, sh, sn)
 
 
 def _workspace(fn, desc, device):
     n = C.c_size_t()
     _lib.check(fn(C.byref(desc), C.byref(n)))
-    return (torch.empty(n.value, dtype=torch.uint8, device=device) if n.value else None), n.value
+    if not n.value:
+        return None, None, 0
+    ws = torch.empty(n.value, dtype=torch.uint8, device=device)
+    return ws, ws.data_ptr(), n.value
 
 
 # ------------------------------------------------------------------------------------------------------------- attention
 def _attn_desc(q, k, v, key_mask, causal, scale, what):
-    for name, t in (("q", q), ("k", k), ("v", v)):
-        if not torch.is_tensor(t) or t.dim() != 4:
-            raise ValueError(f"{what}: {name} must be a [batch, heads, length, channels] tensor")
+    for t in (q, k, v):
+        if not isinstance(t, torch.Tensor) or t.dim() != 4:
+            raise ValueError(f"{what}: q, k and v must be [batch, heads, length, channels] tensors")
     dt = _dtype(q, what)
     B, H, Tq, D = q.shape
     Hkv, Tk = k.shape[1], k.shape[2]
@@ -129,9 +144,10 @@ def _attn_desc(q, k, v, key_mask, causal, scale, what):
         if key_mask.device != q.device:
             raise ValueError(f"{what}: key_mask is on {key_mask.device}, expected {q.device}")
         key_mask = key_mask.contiguous()
-    _lib.require_gpu(q, f"{what} q")
+    if not q.is_cuda:
+        _lib.require_gpu(q, f"{what} q")
     _same(q, what, k=k, v=v)
-    return _lib.AttnDesc(dt, B, H, Hkv, Tq, Tk, D, int(bool(causal)), scale), key_mask
+    return _lib.AttnDesc(dt, B, H, Hkv, Tq, Tk, D, int(bool(causal)), scale), key_mask, (4 if dt == 0 else 8)
 
 
 def _like_rows(t: torch.Tensor) -> torch.Tensor:
@@ -140,45 +156,46 @@ def _like_rows(t: torch.Tensor) -> torch.Tensor:
     return torch.empty(B, T, H, D, dtype=t.dtype, device=t.device).transpose(1, 2)
 
 
-@torch.no_grad()
 def attention_forward(q, k, v, key_mask=None, causal=False, scale=None):
     """(out, lse): out [B, H, Tq, D] = softmax(scale q k^T) v, lse fp32 [B, H, Tq] = the natural logarithm of each row's sum of exponentials.
 
     q [B, H, Tq, D]; k, v [B, Hkv, Tk, D] with H a multiple of Hkv (query head h reads head h // (H // Hkv)); D a multiple of 8 up to 128.
     key_mask [B, Tk], true = masked (whatever masked keys and values hold, NaN included, is never used); causal: query i sees keys up to
     i + Tk - Tq; scale defaults to D ** -0.5.  A row that sees no key is 0 (lse -inf).  Any strides; channels that are not contiguous or not
-    16-byte aligned are copied first."""
-    desc, key_mask = _attn_desc(q, k, v, key_mask, causal, scale, "attention")
-    q, k, v = _aligned(q), _aligned(k), _aligned(v)
+    16-byte aligned are copied first.  No autograd graph (`attention` builds one)."""
+    desc, key_mask, vec = _attn_desc(q, k, v, key_mask, causal, scale, "attention")
+    (q, aq), (k, ak), (v, av) = _arg(q, vec), _arg(k, vec), _arg(v, vec)
+    device = q.device
     out = _like_rows(q)
-    lse = torch.empty(q.shape[:3], dtype=torch.float32, device=q.device)
-    h, lib = _handle(q.device), _lib.lib()
-    ws, n = _workspace(lib.fdx_attn_forward_workspace, desc, q.device)
+    lse = torch.empty(q.shape[:3], dtype=torch.float32, device=device)
+    h, lib = _handle(device), _lib.lib()
+    ws, wp, n = _workspace(lib.fdx_attn_forward_workspace, desc, device)
     with h.lock:
-        _lib.check(lib.fdx_attn_forward(h.h, C.byref(desc), C.byref(_bht(q)), C.byref(_bht(k)), C.byref(_bht(v)), _lib.ptr(key_mask),
-                                        C.byref(_bht(out)), _lib.ptr(lse), _lib.ptr(ws), n, _lib.stream_ptr(q.device)), h.h)
+        rc = lib.fdx_attn_forward(h.h, desc, aq, ak, av, None if key_mask is None else key_mask.data_ptr(), _arg(out, vec)[1], lse.data_ptr(), wp, n, _stream(h))
+        if rc:
+            _lib.check(rc, h.h)
     return out, lse
 
 
-@torch.no_grad()
 def attention_backward(grad_out, q, k, v, out, lse, key_mask=None, causal=False, scale=None):
     """(dq, dk, dv) of `attention_forward` called with the same arguments, from grad_out and its results.  dk / dv are summed over the query
     heads that share a key / value head; masked keys get 0, rows that see no key give 0 whatever grad_out holds there."""
-    desc, key_mask = _attn_desc(q, k, v, key_mask, causal, scale, "attention_backward")
+    desc, key_mask, vec = _attn_desc(q, k, v, key_mask, causal, scale, "attention_backward")
     _same(q, "attention_backward", grad_out=grad_out, out=out)
     if grad_out.shape != q.shape or out.shape != q.shape:
         raise ValueError(f"attention_backward: grad_out {tuple(grad_out.shape)} and out {tuple(out.shape)} must have q's shape {tuple(q.shape)}")
     if lse.shape != q.shape[:3] or lse.dtype != torch.float32 or lse.device != q.device:
         raise ValueError(f"attention_backward: lse must be the forward's float32 {tuple(q.shape[:3])} on {q.device}")
-    grad_out, q, k, v, out = (_aligned(t) for t in (grad_out, q, k, v, out))
+    (grad_out, ag), (q, aq), (k, ak), (v, av), (out, ao) = (_arg(t, vec) for t in (grad_out, q, k, v, out))
     lse = lse.contiguous()
     dq, dk, dv = _like_rows(q), _like_rows(k), _like_rows(v)
     h, lib = _handle(q.device), _lib.lib()
-    ws, n = _workspace(lib.fdx_attn_backward_workspace, desc, q.device)
+    ws, wp, n = _workspace(lib.fdx_attn_backward_workspace, desc, q.device)
     with h.lock:
-        _lib.check(lib.fdx_attn_backward(h.h, C.byref(desc), *(C.byref(_bht(t)) for t in (grad_out, q, k, v, out)), _lib.ptr(lse),
-                                         _lib.ptr(key_mask), *(C.byref(_bht(t)) for t in (dq, dk, dv)), _lib.ptr(ws), n,
-                                         _lib.stream_ptr(q.device)), h.h)
+        rc = lib.fdx_attn_backward(h.h, desc, ag, aq, ak, av, ao, lse.data_ptr(), None if key_mask is None else key_mask.data_ptr(),
+                                   _arg(dq, vec)[1], _arg(dk, vec)[1], _arg(dv, vec)[1], wp, n, _stream(h))
+        if rc:
+            _lib.check(rc, h.h)
     return dq, dk, dv
 
 
@@ -221,8 +238,7 @@ def _packed_rows(t: Optional[torch.Tensor]) -> Optional[torch.Tensor]:
     """Contiguous and 16-byte aligned (a copy where it is not)."""
     if t is None or t.numel() == 0:
         return t
-    t = t.contiguous()
-    return t if t.data_ptr() % 16 == 0 else t.clone()
+    return t if t.is_contiguous() and not t.data_ptr() & 15 else _copy(t)
 
 
 def _norm_args(x, block, gate, residual_scale, post_norm, pre_norm, kind, eps, what):
@@ -261,12 +277,12 @@ def _norm_args(x, block, gate, residual_scale, post_norm, pre_norm, kind, eps, w
             rows = max(x.shape[1], 1)
         else:
             raise ValueError(f"{what}: gate {tuple(gate.shape)} is none of [channels], [batch, channels], [batch, 1, channels] and x's {tuple(x.shape)}")
-    for name, t in (("x", x), ("block", block), ("gate", gate), ("a norm's weight or bias", next((p for p in params if p is not None), None))):
-        if t is not None:
-            _lib.require_gpu(t, f"{what} {name}")
+    device = x.device
     for t in (block, gate, *params):
-        if t is not None and t.device != x.device:
-            raise ValueError(f"{what}: tensors on {t.device} and {x.device}")
+        if t is not None and t.device != device:
+            raise ValueError(f"{what}: tensors on {t.device} and {device}")
+    if not x.is_cuda:
+        _lib.require_gpu(x, f"{what} x")
     if block.dtype != x.dtype:
         raise ValueError(f"{what}: block is {block.dtype}, x {x.dtype}")
     desc = _lib.ResnormDesc(dt, _lib.DTYPES[next(iter(pdt))], dt if gate is None else _lib.DTYPES[gate.dtype], N, C_, rows, _KINDS[kind],
@@ -274,7 +290,6 @@ def _norm_args(x, block, gate, residual_scale, post_norm, pre_norm, kind, eps, w
     return desc, [_packed_rows(p) for p in params]
 
 
-@torch.no_grad()
 def residual_norm_forward(x, block, gate=None, residual_scale=1.0, post_norm=None, pre_norm=None, kind="layer", eps=1e-5):
     """(h, y, stats): h = residual_scale * x + gate * post_norm(block), y = pre_norm(h) (None without one), stats for the backward pass.
 
@@ -289,12 +304,11 @@ def residual_norm_forward(x, block, gate=None, residual_scale=1.0, post_norm=Non
     if x.numel():
         h, lib = _handle(x.device), _lib.lib()
         with h.lock:
-            _lib.check(lib.fdx_resnorm_forward(h.h, C.byref(desc), *(_lib.ptr(t) for t in (x, block, gate, pw, pb, nw, nb, h_out, y, stats)),
-                                               _lib.stream_ptr(x.device)), h.h)
+            _lib.check(lib.fdx_resnorm_forward(h.h, desc, *(_p(t) for t in (x, block, gate, pw, pb, nw, nb, h_out, y, stats)),
+                                               _stream(h)), h.h)
     return h_out, y, stats
 
 
-@torch.no_grad()
 def residual_norm_backward(grad_h, grad_y, x, block, stats, gate=None, residual_scale=1.0, post_norm=None, pre_norm=None, kind="layer", eps=1e-5):
     """`ResidualNormGrads` from the gradients of h and y (either may be None) and the forward's arguments and stats.  Where there is no gate, no post norm and
     residual_scale is 1, dx and dblock are equal and are ONE tensor.  The gate's gradient has the gate's shape."""
@@ -317,10 +331,10 @@ def residual_norm_backward(grad_h, grad_y, x, block, stats, gate=None, residual_
                 t.zero_()
     else:
         h, lib = _handle(x.device), _lib.lib()
-        ws, n = _workspace(lib.fdx_resnorm_backward_workspace, desc, x.device)
+        ws, wp, n = _workspace(lib.fdx_resnorm_backward_workspace, desc, x.device)
         with h.lock:
-            _lib.check(lib.fdx_resnorm_backward(h.h, C.byref(desc), *(_lib.ptr(t) for t in (grad_h, grad_y, x, block, gate_c, pw, pb, nw, nb, stats, dx, dblock,
-                                                                                           dgate, *grads, ws)), n, _lib.stream_ptr(x.device)), h.h)
+            _lib.check(lib.fdx_resnorm_backward(h.h, desc, *(_p(t) for t in (grad_h, grad_y, x, block, gate_c, pw, pb, nw, nb, stats, dx, dblock,
+                                                                                           dgate, *grads)), wp, n, _stream(h)), h.h)
     return ResidualNormGrads(dx, dblock, dgate, *grads)
 
 
@@ -378,23 +392,22 @@ def _new_packed(x: torch.Tensor) -> Packed8:
                    torch.empty((*x.shape[:-1], (x.shape[-1] + 31) // 32), dtype=torch.uint8, device=x.device))
 
 
-@torch.no_grad()
 def pack8(x) -> Packed8:
     """x [..., C] in 8 bits.  Each group of 32 channels shares the smallest power of two 2^k, k >= -126, with max|x| <= 127 * 2^k; codes are x / 2^k rounded to
     nearest even, so the error is at most half of 2^k (at the very top of fp32's range, k = 122, codes end at 63 so that no finite value reads back
     infinite).  A group with an infinity or NaN reads back as NaN."""
     N, C_ = _rows_of(x, "pack8", "x")
     dt = _dtype(x, "pack8")
-    _lib.require_gpu(x, "pack8 x")
+    if not x.is_cuda:
+        _lib.require_gpu(x, "pack8 x")
     x = _packed_rows(x)
     p = _new_packed(x)
     h = _handle(x.device)
     with h.lock:
-        _lib.check(_lib.lib().fdx_pack8(h.h, dt, _lib.ptr(x), N, C_, _lib.ptr(p.codes), _lib.ptr(p.exponents), _lib.stream_ptr(x.device)), h.h)
+        _lib.check(_lib.lib().fdx_pack8(h.h, dt, _p(x), N, C_, _p(p.codes), _p(p.exponents), _stream(h)), h.h)
     return p
 
 
-@torch.no_grad()
 def unpack8(packed: Packed8, dtype=torch.float32) -> torch.Tensor:
     """What the codes stand for (exact in float32 and bfloat16; in float16 at most 65504)."""
     p = _packed_ok(packed, "unpack8")
@@ -403,12 +416,11 @@ def unpack8(packed: Packed8, dtype=torch.float32) -> torch.Tensor:
     out = torch.empty(p.codes.shape, dtype=dtype, device=p.codes.device)
     h = _handle(out.device)
     with h.lock:
-        _lib.check(_lib.lib().fdx_unpack8(h.h, _lib.DTYPES[dtype], _lib.ptr(p.codes), _lib.ptr(p.exponents), *_rows_of(p.codes, "unpack8", "codes"), _lib.ptr(out),
-                                          _lib.stream_ptr(out.device)), h.h)
+        _lib.check(_lib.lib().fdx_unpack8(h.h, _lib.DTYPES[dtype], _p(p.codes), _p(p.exponents), *_rows_of(p.codes, "unpack8", "codes"), _p(out),
+                                          _stream(h)), h.h)
     return out
 
 
-@torch.no_grad()
 def linear8_weight_grad(dy, packed: Packed8, bias=True, dtype=None):
     """(dw, db) of y = x w^T + b from dy [..., out] and x kept as `pack8(x)` [..., in]: dw [out, in] = sum over rows of dy x8, db [out] = sum of dy (None if not
     `bias`).  Products are exact and summed in fp32; results in `dtype` (default dy's)."""
@@ -431,12 +443,11 @@ def linear8_weight_grad(dy, packed: Packed8, bias=True, dtype=None):
     _lib.check(lib.fdx_linear8_weight_grad_workspace(dt, N, O, I, C.byref(n)))
     ws = torch.empty(n.value, dtype=torch.uint8, device=dy.device)
     with h.lock:
-        _lib.check(lib.fdx_linear8_weight_grad(h.h, dt, _lib.ptr(dy), _lib.ptr(p.codes), _lib.ptr(p.exponents), N, O, I, _lib.DTYPES[dtype], _lib.ptr(dw),
-                                               _lib.ptr(db), _lib.ptr(ws), n.value, _lib.stream_ptr(dy.device)), h.h)
+        _lib.check(lib.fdx_linear8_weight_grad(h.h, dt, _p(dy), _p(p.codes), _p(p.exponents), N, O, I, _lib.DTYPES[dtype], _p(dw),
+                                               _p(db), _p(ws), n.value, _stream(h)), h.h)
     return dw, db
 
 
-@torch.no_grad()
 def gelu8_forward(x):
     """(gelu(x), pack8(x)) in one pass; GELU in its erf form, from x itself."""
     N, C_ = _rows_of(x, "gelu8", "x")
@@ -446,11 +457,10 @@ def gelu8_forward(x):
     y, p = torch.empty_like(x), _new_packed(x)
     h = _handle(x.device)
     with h.lock:
-        _lib.check(_lib.lib().fdx_gelu8_forward(h.h, dt, _lib.ptr(x), N, C_, _lib.ptr(y), _lib.ptr(p.codes), _lib.ptr(p.exponents), _lib.stream_ptr(x.device)), h.h)
+        _lib.check(_lib.lib().fdx_gelu8_forward(h.h, dt, _p(x), N, C_, _p(y), _p(p.codes), _p(p.exponents), _stream(h)), h.h)
     return y, p
 
 
-@torch.no_grad()
 def gelu8_backward(dy, packed: Packed8):
     """dy * gelu'(x8), x8 what `packed` stands for."""
     N, C_ = _rows_of(dy, "gelu8_backward", "dy")
@@ -465,7 +475,7 @@ def gelu8_backward(dy, packed: Packed8):
     dx = torch.empty_like(dy)
     h = _handle(dy.device)
     with h.lock:
-        _lib.check(_lib.lib().fdx_gelu8_backward(h.h, dt, _lib.ptr(dy), _lib.ptr(p.codes), _lib.ptr(p.exponents), N, C_, _lib.ptr(dx), _lib.stream_ptr(dy.device)), h.h)
+        _lib.check(_lib.lib().fdx_gelu8_backward(h.h, dt, _p(dy), _p(p.codes), _p(p.exponents), N, C_, _p(dx), _stream(h)), h.h)
     return dx
 
 
