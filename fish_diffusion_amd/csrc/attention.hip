@@ -21,6 +21,13 @@
 
 using namespace fdx;
 
+#ifndef FWD_W
+#define FWD_W(T, DH) 1
+#define DQ_W(T, DH) 1
+#define DKV_W(T, DH) 1
+#define DKV_RT(T, DH) 64
+#define DQ_KT(T, DH) 64
+#endif
 namespace {
 
 struct Str { long b, h, t; };
@@ -57,24 +64,63 @@ __device__ inline int key_end(const AttnArgs& a, int r0, int r1) {
   return max(0, min(a.Tk, t + a.off + 1));
 }
 
-// TK rows of DH elements on their way from memory to LDS, in registers of the 256 threads
-template <typename T, int DH, int TK> struct Stage {
+__device__ __attribute__((aligned(16))) unsigned g_zero[4];   // where rows that do not exist are read
+
+// TK rows of DH elements from memory straight to LDS (global_load_lds_dwordx4: a wave-instruction lands 64 chunks in a row at a wave-uniform address, so
+// the tile's swizzle is applied to the SOURCE address).  No staging registers: that is what lets two workgroups share a CU.  The loads are counted by
+// the wait in front of the barrier that publishes the tile (landed()); written as asm because with the builtin in flight the compiler waits for every
+// LDS read.  A load has no register output, so nothing can overwrite what is in flight.
+template <typename T, int DH, int TK> struct Fill {
   typedef Tile<T, DH> Tl;
-  static constexpr int NV = TK * Tl::CPR / 256;
-  static_assert(NV * 256 == TK * Tl::CPR, "whole vectors per thread");
-  uint4 r[NV];
-  static __device__ inline int row(int i) { return ((int)threadIdx.x + 256 * i) / Tl::CPR; }
-  static __device__ inline int chunk(int i) { return ((int)threadIdx.x + 256 * i) % Tl::CPR; }
-  template <typename F> __device__ inline void load(F&& src, int D) {   // src(row, i): row's address or null (zeros)
+  static constexpr int N = TK * Tl::CPR / 256, RPI = 64 / Tl::CPR > 0 ? 64 / Tl::CPR : 1;   // wave-instructions per wave, rows each covers
+  static_assert(N * 256 == TK * Tl::CPR && 64 % Tl::CPR == 0, "whole rows per instruction");
+  template <typename F> static __device__ inline void issue(uint4* lds, F&& src, int D) {   // src(row): its address, or null (zeros)
+    const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), lane = threadIdx.x & 63;
+    const unsigned base = (unsigned)(size_t)(__attribute__((address_space(3))) uint4*)lds;
 #pragma unroll
-    for (int i = 0; i < NV; ++i) {
-      const T* p = src(row(i), i);
-      r[i] = p && chunk(i) * Elem<T>::VEC < D ? *reinterpret_cast<const uint4*>(p + chunk(i) * Elem<T>::VEC) : uint4{0, 0, 0, 0};
+    for (int i = 0; i < N; ++i) {
+      const int row = (i * 4 + wave) * RPI + lane / Tl::CPR, c = (lane % Tl::CPR) ^ Tl::swz(row);
+      const T* p = src(row);
+      const void* from = p && c * Elem<T>::VEC < D ? static_cast<const void*>(p + c * Elem<T>::VEC) : g_zero;
+      const unsigned to = base + (unsigned)(i * 4 + wave) * 1024u;
+      unsigned keep;
+      asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off\n\ts_mov_b32 m0, %0"
+                   : "=&s"(keep) : "v"(from), "s"(to) : "memory");
     }
   }
-  __device__ inline void store(uint4* lds) const {
+};
+// stages of a tile pair of `bytes`: two (a step's loads fly while the one before is computed) where two workgroups still fit on a CU, else one (the
+// other workgroup's products cover the loads)
+constexpr int stages_of(int bytes) { return 2 * bytes <= 80 * 1024 ? 2 : 1; }
+
+// every wave's loads into LDS have landed, and every wave is done with the tile before
+__device__ inline void landed() {
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+  __syncthreads();
+}
+
+// which of a step's TK rows exist and are not masked, in every wave: loaded one step before it is needed
+template <int TK> struct RowBits {
+  static constexpr int N = (TK + 63) / 64;
+  unsigned char m[N];
+  unsigned long long bits[N];
+  __device__ inline void load(const uint8_t* mask, int first, int end, int lane) {
 #pragma unroll
-    for (int i = 0; i < NV; ++i) lds[Tl::at(row(i), chunk(i))] = r[i];
+    for (int i = 0; i < N; ++i) {
+      const int k = first + 64 * i + lane;
+      m[i] = k >= end || (TK < 64 && lane >= TK) ? 1 : mask ? mask[k] : 0;
+    }
+  }
+  __device__ inline void vote() {
+#pragma unroll
+    for (int i = 0; i < N; ++i) bits[i] = __ballot(m[i] == 0);
+  }
+  __device__ inline bool has(int row) const { return (bits[N == 1 ? 0 : row >> 6] >> (row & 63)) & 1; }
+  __device__ inline bool any() const {
+    unsigned long long o = 0;
+#pragma unroll
+    for (int i = 0; i < N; ++i) o |= bits[i];
+    return o != 0;
   }
 };
 
@@ -86,6 +132,28 @@ template <typename T, int DH> __device__ inline void load_rows(typename Elem<T>:
     f[s] = __builtin_bit_cast(typename Elem<T>::frag, p && e < D ? *reinterpret_cast<const uint4*>(p + e) : uint4{0, 0, 0, 0});
   }
 }
+
+// The wave's own column operands either in registers or, where accumulators and two of them would not leave room for two waves per SIMD (16-bit types,
+// head size 128), parked in LDS in lane order and read back at every use.
+template <typename T, int DH, bool PARK> struct Own {
+  typedef typename Elem<T>::frag frag;
+  static constexpr int NS = DH / Elem<T>::KS;
+  frag f[PARK ? 1 : NS];
+  uint4* at;
+  __device__ inline void park(uint4* lds, int wave, int lane) { at = lds + wave * NS * 64 + lane; }
+  __device__ inline void set(const frag* v) {
+#pragma unroll
+    for (int s = 0; s < NS; ++s) {
+      if constexpr (PARK) at[s * 64] = __builtin_bit_cast(uint4, v[s]);
+      else f[s] = v[s];
+    }
+  }
+  __device__ inline frag get(int s) const {
+    if constexpr (PARK) return __builtin_bit_cast(frag, at[s * 64]);
+    else return f[s];
+  }
+};
+template <typename T, int DH> constexpr bool parked() { return sizeof(T) == 2 && DH == 128; }
 
 template <typename T> __device__ inline void store4(T* p, float a, float b, float c, float d) {
   typedef T v4 __attribute__((ext_vector_type(4)));
@@ -128,14 +196,14 @@ template <> struct PShift<f16_t> { static constexpr float log2 = 14.f, back = 0x
 // WQ waves take 32 rows each, the other factor of the 4 waves (WK) shares those rows and takes KT keys each of every step; their
 // (max, sum, O) meet in LDS at the end.  Online softmax: running maximum m of the raw scores, P = exp2(c s - c m).
 template <typename T, int DH, int WQ, int KT>
-__global__ __launch_bounds__(256) void k_attn_fwd(AttnArgs a) {
+__global__ __launch_bounds__(256, FWD_W(T, DH)) void k_attn_fwd(AttnArgs a) {
   typedef Tile<T, DH> Tl;
   typedef typename Elem<T>::frag frag;
   constexpr int KS = Elem<T>::KS, WK = 4 / WQ, TK = KT * WK, NS = DH / KS, MT = DH / 32, NU = KT / 32, NP = 32 / KS;
   constexpr int kTile = TK * Tl::CPR, kMerge = WK > 1 ? WK * 32 * DH / 4 : 0;   // in 16-byte units
-  __shared__ uint4 smem[2 * kTile > kMerge ? 2 * kTile : kMerge];
+  constexpr int S = stages_of(32 * kTile);
+  __shared__ uint4 smem[2 * S * kTile > kMerge ? 2 * S * kTile : kMerge];       // S stages of K and V
   __shared__ float ml[2][4][32];
-  uint4 *const lk = smem, *const lv = smem + kTile;
   int bh, tile, split;
   decode(a, bh, tile, split);
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wq = wave / WK, wk = wave % WK, hi = lane >> 5;
@@ -153,24 +221,40 @@ __global__ __launch_bounds__(256) void k_attn_fwd(AttnArgs a) {
   for (int m = 0; m < MT; ++m) acc[m] = f32x16{0};
   float mx = -inf(), l = 0.f;
 
-  Stage<T, DH, TK> sk, sv;
-  unsigned long long bits_next = 0;
-  auto fetch = [&](int st) {
+  RowBits<TK> rb;
+  int stage = 0;
+  auto fetch = [&](int st) {   // (masked rows enter as zeros: 0 * NaN never happens)
     const int k0 = st * TK;
-    const int kk = k0 + wk * KT + lane;
-    bits_next = __ballot(lane < KT && kk < a.Tk && !(mask && mask[min(kk, a.Tk - 1)]));
-    auto ok = [&](int row) { const int key = k0 + row; return key < a.Tk && !(mask && mask[key]); };   // masked rows enter as zeros: 0 * NaN never happens
-    sk.load([&](int row, int) { return ok(row) ? K + (long)(k0 + row) * a.sk.t : nullptr; }, a.D);
-    sv.load([&](int row, int) { return ok(row) ? V + (long)(k0 + row) * a.sv.t : nullptr; }, a.D);
+    uint4* const to = smem + stage * 2 * kTile;
+    Fill<T, DH, TK>::issue(to, [&](int row) { return rb.has(row) ? K + (long)(k0 + row) * a.sk.t : nullptr; }, a.D);
+    Fill<T, DH, TK>::issue(to + kTile, [&](int row) { return rb.has(row) ? V + (long)(k0 + row) * a.sv.t : nullptr; }, a.D);
   };
-  if (split < steps) fetch(split);
+  if (split < steps) {
+    rb.load(mask, split * TK, a.Tk, lane);
+    rb.vote();
+    if (S == 2) {
+      if (rb.any()) fetch(split);
+      rb.load(mask, (split + a.splits) * TK, a.Tk, lane);
+    }
+  }
   for (int st = split; st < steps; st += a.splits) {
-    __syncthreads();
-    sk.store(lk);
-    sv.store(lv);
-    const unsigned long long bits = bits_next;
-    __syncthreads();
-    if (st + a.splits < steps) fetch(st + a.splits);
+    if constexpr (S == 1) {
+      __syncthreads();
+      if (rb.any()) fetch(st);
+      rb.load(mask, (st + a.splits) * TK, a.Tk, lane);
+    }
+    landed();
+    const uint4 *const lk = smem + stage * 2 * kTile, *const lv = lk + kTile;
+    unsigned long long bits = rb.bits[wk * KT / 64];
+    if constexpr (KT == 32) bits = (bits >> (wk * KT % 64)) & 0xffffffffull;
+    if constexpr (S == 2) stage ^= 1;
+    if (st + a.splits < steps) {
+      rb.vote();
+      if constexpr (S == 2) {
+        if (rb.any()) fetch(st + a.splits);
+        rb.load(mask, (st + 2 * a.splits) * TK, a.Tk, lane);
+      }
+    }
     if (bits == 0) continue;   // (the wave's keys are all masked; the barriers are outside)
     f32x16 s[NU];
 #pragma unroll
@@ -238,7 +322,7 @@ __global__ __launch_bounds__(256) void k_attn_fwd(AttnArgs a) {
   } else {
     static_assert(WQ == 1, "the waves that share rows are all four");
     if (hi == 0) { ml[0][wk][lane] = mc; ml[1][wk][lane] = l; }
-    __syncthreads();   // also: the last tile has been read
+    landed();   // also: the last tile has been read (and nothing is on its way)
     float M = -inf(), L = 0.f;
 #pragma unroll
     for (int w = 0; w < WK; ++w) M = fmaxf(M, ml[0][w][lane & 31]);
@@ -318,15 +402,20 @@ struct RunScale {
 };
 
 // dq, and delta for the dk / dv pass (which runs behind this one).  Same split of rows and keys over the waves as the forward.
+// 16-bit types: delta = do.o sees o as it was rounded, off by d.  P(dP - delta) sums to 0 over a row, so the sum r of what was computed IS d, up to
+// fp32: dq = scale (sum dS k - r sum P k), at the price of one more product whose operand is in place, and the dk / dv pass gets delta + r.
 template <typename T, int DH, int WQ, int KT>
-__global__ __launch_bounds__(256) void k_attn_dq(AttnArgs a) {
+__global__ __launch_bounds__(256, DQ_W(T, DH)) void k_attn_dq(AttnArgs a) {
   typedef Tile<T, DH> Tl;
   typedef typename Elem<T>::frag frag;
-  constexpr bool kScaled = DtOf<T>::v == DT_F16;
+  constexpr bool kScaled = DtOf<T>::v == DT_F16, kMend = sizeof(T) == 2;
   constexpr int KS = Elem<T>::KS, WK = 4 / WQ, TK = KT * WK, NS = DH / KS, MT = DH / 32, NU = KT / 32, NP = 32 / KS;
   constexpr int kTile = TK * Tl::CPR, kMerge = WK > 1 ? WK * 32 * DH / 4 : 0;
-  __shared__ uint4 smem[2 * kTile > kMerge ? 2 * kTile : kMerge];
-  uint4 *const lk = smem, *const lv = smem + kTile;
+  constexpr int S = stages_of(32 * kTile);
+  __shared__ uint4 smem[2 * S * kTile > kMerge ? 2 * S * kTile : kMerge];
+  __shared__ float rest[4][32];
+  constexpr bool PARK = parked<T, DH>();
+  __shared__ uint4 own[PARK ? 4 * NS * 64 : 1];
   int bh, tile, split;
   decode(a, bh, tile, split);
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wq = wave / WK, wk = wave % WK, hi = lane >> 5;
@@ -338,47 +427,70 @@ __global__ __launch_bounds__(256) void k_attn_dq(AttnArgs a) {
   const T* const K = static_cast<const T*>(a.k) + b * a.sk.b + hk * a.sk.h;
   const T* const V = static_cast<const T*>(a.v) + b * a.sv.b + hk * a.sv.h;
   const uint8_t* const mask = a.mask ? a.mask + (long)b * a.Tk : nullptr;
-  frag qf[NS], gf[NS];
+  RowBits<TK> rb;
+  int stage = 0;
+  auto fetch = [&](int st) {
+    const int k0 = st * TK;
+    uint4* const to = smem + stage * 2 * kTile;
+    Fill<T, DH, TK>::issue(to, [&](int row) { return rb.has(row) ? K + (long)(k0 + row) * a.sk.t : nullptr; }, a.D);
+    Fill<T, DH, TK>::issue(to + kTile, [&](int row) { return rb.has(row) ? V + (long)(k0 + row) * a.sv.t : nullptr; }, a.D);
+  };
+  if (split < steps) {
+    rb.load(mask, split * TK, a.Tk, lane);
+    rb.vote();
+    if (S == 2) {
+      if (rb.any()) fetch(split);
+      rb.load(mask, (split + a.splits) * TK, a.Tk, lane);
+    }
+  }
+  frag qf[NS];
+  Own<T, DH, PARK> gf;
   load_rows<T, DH>(qf, static_cast<const T*>(a.q) + b * a.sq.b + h * a.sq.h + t * a.sq.t, a.D, lane);
-  load_rows<T, DH>(gf, static_cast<const T*>(a.go) + b * a.sgo.b + h * a.sgo.h + t * a.sgo.t, a.D, lane);
   const float lse = a.lse[(long)bh * a.R + rc];
   const bool empty = lse == -inf();
   float delta = 0.f;
   {
-    frag of[NS];
+    frag of[NS], go[NS];
+    load_rows<T, DH>(go, static_cast<const T*>(a.go) + b * a.sgo.b + h * a.sgo.h + t * a.sgo.t, a.D, lane);
     load_rows<T, DH>(of, static_cast<const T*>(a.o) + b * a.so.b + h * a.so.h + t * a.so.t, a.D, lane);
 #pragma unroll
     for (int s = 0; s < NS; ++s)
 #pragma unroll
-      for (int j = 0; j < Elem<T>::VEC; ++j) delta = __builtin_fmaf((float)gf[s][j], (float)of[s][j], delta);
+      for (int j = 0; j < Elem<T>::VEC; ++j) delta = __builtin_fmaf((float)go[s][j], (float)of[s][j], delta);
     delta += other_half(delta);
     if (empty) delta = 0.f;   // (whatever stands in do there)
+    gf.park(own, wave, lane);
+    gf.set(go);
   }
-  if (wk == 0 && hi == 0 && split == 0 && r < a.R) a.delta[(long)bh * a.R + r] = delta;
   const float L = empty ? inf() : lse * kLog2e;   // exp2(x - inf) = 0
-  f32x16 acc[MT];
+  f32x16 acc[MT], pk[kMend ? MT : 1];
 #pragma unroll
   for (int m = 0; m < MT; ++m) acc[m] = f32x16{0};
+  if constexpr (kMend) {
+#pragma unroll
+    for (int m = 0; m < MT; ++m) pk[m] = f32x16{0};
+  }
+  float left = 0.f;   // sum of dS over the row
   RunScale rs;
 
-  Stage<T, DH, TK> sk, sv;
-  unsigned long long bits_next = 0;
-  auto fetch = [&](int st) {
-    const int k0 = st * TK;
-    const int kk = k0 + wk * KT + lane;
-    bits_next = __ballot(lane < KT && kk < a.Tk && !(mask && mask[min(kk, a.Tk - 1)]));
-    auto ok = [&](int row) { const int key = k0 + row; return key < a.Tk && !(mask && mask[key]); };
-    sk.load([&](int row, int) { return ok(row) ? K + (long)(k0 + row) * a.sk.t : nullptr; }, a.D);
-    sv.load([&](int row, int) { return ok(row) ? V + (long)(k0 + row) * a.sv.t : nullptr; }, a.D);
-  };
-  if (split < steps) fetch(split);
   for (int st = split; st < steps; st += a.splits) {
-    __syncthreads();
-    sk.store(lk);
-    sv.store(lv);
-    const unsigned long long bits = bits_next;
-    __syncthreads();
-    if (st + a.splits < steps) fetch(st + a.splits);
+    if constexpr (S == 1) {
+      __syncthreads();
+      if (rb.any()) fetch(st);
+      rb.load(mask, (st + a.splits) * TK, a.Tk, lane);
+    }
+    landed();
+    const uint4 *const lk = smem + stage * 2 * kTile, *const lv = lk + kTile;
+    unsigned long long bits = rb.bits[wk * KT / 64];
+    if constexpr (KT == 32) bits = (bits >> (wk * KT % 64)) & 0xffffffffull;
+    if constexpr (S == 2) stage ^= 1;
+    if (st + a.splits < steps) {
+      rb.vote();
+      if constexpr (S == 2) {
+        if (rb.any()) fetch(st + a.splits);
+        rb.load(mask, (st + 2 * a.splits) * TK, a.Tk, lane);
+      }
+    }
     if (bits == 0) continue;
     const int rel = lim - (st * TK + wk * KT);
     const unsigned long long full = KT == 64 ? ~0ull : (1ull << KT) - 1;
@@ -391,47 +503,137 @@ __global__ __launch_bounds__(256) void k_attn_dq(AttnArgs a) {
 #pragma unroll
       for (int i = 0; i < NS; ++i) {
         s = Elem<T>::mma(Tl::row(lk, kr + (lane & 31), 2 * i + hi), qf[i], s);
-        dp = Elem<T>::mma(Tl::row(lv, kr + (lane & 31), 2 * i + hi), gf[i], dp);
+        dp = Elem<T>::mma(Tl::row(lv, kr + (lane & 31), 2 * i + hi), gf.get(i), dp);
       }
 #pragma unroll
-      for (int e = 0; e < 16; ++e) s[e] = exp2_(__builtin_fmaf(s[e], a.c, -L)) * (dp[e] - delta);
+      for (int e = 0; e < 16; ++e) s[e] = exp2_(__builtin_fmaf(s[e], a.c, PShift<T>::log2 - L));
       if (!whole) {
         const unsigned w = (unsigned)(ok >> (32 * u)) >> (4 * hi);
 #pragma unroll
-        for (int e = 0; e < 16; ++e) s[e] = (w >> (8 * (e >> 2) + (e & 3))) & 1 ? s[e] : 0.f;
+        for (int e = 0; e < 16; ++e) {
+          const bool in = (w >> (8 * (e >> 2) + (e & 3))) & 1;
+          s[e] = in ? s[e] : 0.f;
+          dp[e] = in ? dp[e] : delta;
+        }
       }
-      if constexpr (kScaled) rs.fit<MT>(s, acc);
+#pragma unroll
+      for (int e = 0; e < 16; ++e) dp[e] = s[e] * PShift<T>::back * (dp[e] - delta);
+      if constexpr (kMend) {
+#pragma unroll
+        for (int e = 0; e < 16; ++e) left += dp[e];
+      }
+      if constexpr (kScaled) rs.fit<MT>(dp, acc);
 #pragma unroll
       for (int p = 0; p < NP; ++p) {
-        const frag df = acc_frag<T>(s, p);
+        const frag df = acc_frag<T>(dp, p);
+        frag pf;
+        if constexpr (kMend) pf = acc_frag<T>(s, p);
 #pragma unroll
-        for (int m = 0; m < MT; ++m) acc[m] = Elem<T>::mma(Tl::col(lk, kr + KS * p, m, lane), df, acc[m]);
+        for (int m = 0; m < MT; ++m) {
+          const frag kf = Tl::col(lk, kr + KS * p, m, lane);
+          acc[m] = Elem<T>::mma(kf, df, acc[m]);
+          if constexpr (kMend) pk[m] = Elem<T>::mma(kf, pf, pk[m]);
+        }
       }
     }
   }
   float f = a.scale;
   if constexpr (kScaled) f /= rs.s;
+  if constexpr (kMend) left += other_half(left);
+  const float fp = a.scale * PShift<T>::back;   // of pk
   const long prow = ((long)bh * a.splits + split) * a.R;
+  float* const part_pk = a.part + (long)a.B * a.Hkv * a.splits * a.R * a.D;
+  float* const part_r = part_pk + (kMend ? (long)a.B * a.Hkv * a.splits * a.R * a.D : 0);
+  if constexpr (WK > 1) {
+    if constexpr (kMend) {   // the row's sum over the waves
+      if (hi == 0) rest[wk][lane] = left;
+      __syncthreads();
+      left = rest[0][lane & 31] + rest[1][lane & 31] + rest[2][lane & 31] + rest[3][lane & 31];
+    }
+  }
+  if (wk == 0 && hi == 0 && r < a.R) {
+    if (a.splits == 1) a.delta[(long)bh * a.R + r] = delta + left;
+    else {
+      if (split == 0) a.delta[(long)bh * a.R + r] = delta;   // k_attn_join_dq adds the rest
+      if constexpr (kMend) part_r[prow + r] = left;
+    }
+  }
+  const bool whole_row = a.splits == 1;
+  if constexpr (kMend) {
+#pragma unroll
+    for (int m = 0; m < MT; ++m) {
+      acc[m] *= f;
+      if (whole_row) acc[m] -= pk[m] * (fp * left);
+    }
+    f = 1.f;
+  }
   if constexpr (WK == 1) {
     if (r >= a.R) return;
-    if (a.splits > 1) store_cols<float, MT>(a.part + (prow + r) * a.D, acc, f, a.D, lane);
-    else store_cols<T, MT>(static_cast<T*>(a.dq) + b * a.sdq.b + h * a.sdq.h + t * a.sdq.t, acc, f, a.D, lane);
+    if (whole_row) store_cols<T, MT>(static_cast<T*>(a.dq) + b * a.sdq.b + h * a.sdq.h + t * a.sdq.t, acc, f, a.D, lane);
+    else {
+      store_cols<float, MT>(a.part + (prow + r) * a.D, acc, f, a.D, lane);
+      if constexpr (kMend) store_cols<float, MT>(part_pk + (prow + r) * a.D, pk, fp, a.D, lane);
+    }
   } else {
-    __syncthreads();
     float* const red = reinterpret_cast<float*>(smem);
+    auto out = [&](float* part) {   // the waves' blocks in LDS, summed, to the partial rows or to dq
+      for (int i = threadIdx.x; i < 32 * (DH / 4); i += 256) {
+        const int row = i / (DH / 4), d = i % (DH / 4) * 4, rr = r0 + row;
+        if (rr >= a.R || d >= a.D) continue;
+        const f32x4 v = sum_rows<DH>(red, row, d);
+        if (!whole_row) *reinterpret_cast<f32x4*>(part + (prow + rr) * a.D + d) = v;
+        else {
+          const int gg = rr / a.Tq, tt = rr - gg * a.Tq;
+          store4<T>(static_cast<T*>(a.dq) + b * a.sdq.b + (hk * a.G + gg) * a.sdq.h + tt * a.sdq.t + d, v[0], v[1], v[2], v[3]);
+        }
+      }
+    };
+    landed();
     put_rows<DH>(red + wk * 32 * DH, acc, f, lane);
     __syncthreads();
-    for (int i = threadIdx.x; i < 32 * (DH / 4); i += 256) {
-      const int row = i / (DH / 4), d = i % (DH / 4) * 4, rr = r0 + row;
-      if (rr >= a.R || d >= a.D) continue;
-      const f32x4 v = sum_rows<DH>(red, row, d);
-      if (a.splits > 1) *reinterpret_cast<f32x4*>(a.part + (prow + rr) * a.D + d) = v;
-      else {
-        const int gg = rr / a.Tq, tt = rr - gg * a.Tq;
-        store4<T>(static_cast<T*>(a.dq) + b * a.sdq.b + (hk * a.G + gg) * a.sdq.h + tt * a.sdq.t + d, v[0], v[1], v[2], v[3]);
+    out(a.part);
+    if constexpr (kMend) {
+      if (!whole_row) {
+        __syncthreads();
+        put_rows<DH>(red + wk * 32 * DH, pk, fp, lane);
+        __syncthreads();
+        out(part_pk);
       }
     }
   }
+}
+
+// splits of the keys joined for dq (and delta): one wave per row, two channels a lane
+template <typename T> __global__ __launch_bounds__(256) void k_attn_join_dq(AttnArgs a) {
+  constexpr bool kMend = sizeof(T) == 2;
+  const int lane = threadIdx.x & 63;
+  const long row = (long)blockIdx.x * 4 + (threadIdx.x >> 6), rows = (long)a.B * a.Hkv * a.R;
+  if (row >= rows) return;
+  const long bh = row / a.R, r = row - bh * a.R;
+  const float* const part_pk = a.part + rows * a.splits * a.D;
+  const float* const part_r = part_pk + (kMend ? rows * a.splits * a.D : 0);
+  float left = 0.f, o0 = 0.f, o1 = 0.f, p0 = 0.f, p1 = 0.f;
+  for (int s = 0; s < a.splits; ++s) {
+    const long at = (bh * a.splits + s) * a.R + r;
+    if constexpr (kMend) left += part_r[at];
+    if (2 * lane < a.D) {
+      const float2 o = *reinterpret_cast<const float2*>(a.part + at * a.D + 2 * lane);
+      o0 += o.x;
+      o1 += o.y;
+      if constexpr (kMend) {
+        const float2 p = *reinterpret_cast<const float2*>(part_pk + at * a.D + 2 * lane);
+        p0 += p.x;
+        p1 += p.y;
+      }
+    }
+  }
+  const int b = (int)(bh / a.Hkv), hk = (int)(bh % a.Hkv), g = (int)r / a.Tq, t = (int)r - g * a.Tq;
+  if (2 * lane < a.D) {
+    T* p = static_cast<T*>(a.dq) + b * a.sdq.b + (hk * a.G + g) * a.sdq.h + t * a.sdq.t + 2 * lane;
+    p[0] = (T)(o0 - left * p0);
+    p[1] = (T)(o1 - left * p1);
+  }
+  if (kMend && lane == 0) a.delta[row] += left;
 }
 
 // partial sums [B * Hkv][splits][n rows][D] of one gradient joined in split order; rows are (g, t) with G = rows / T heads per kv head
@@ -449,16 +651,18 @@ template <typename T> __global__ __launch_bounds__(256) void k_attn_join_sum(Joi
 
 // dk, dv: WN waves own 32 keys each, the other factor (WR) shares those keys and takes RT rows each of every step
 template <typename T, int DH, int WN, int RT>
-__global__ __launch_bounds__(256) void k_attn_dkv(AttnArgs a) {
+__global__ __launch_bounds__(256, DKV_W(T, DH)) void k_attn_dkv(AttnArgs a) {
   typedef Tile<T, DH> Tl;
   typedef typename Elem<T>::frag frag;
   constexpr bool kScaled = DtOf<T>::v == DT_F16;
   constexpr int KS = Elem<T>::KS, WR = 4 / WN, TR = RT * WR, NS = DH / KS, MT = DH / 32, NU = RT / 32, NP = 32 / KS;
   constexpr int kTile = TR * Tl::CPR, kMerge = WR > 1 ? WR * 32 * DH / 4 : 0;
-  __shared__ uint4 smem[2 * kTile > kMerge ? 2 * kTile : kMerge];
-  __shared__ __attribute__((aligned(16))) float rowL[TR], rowD[TR];
-  __shared__ __attribute__((aligned(16))) int rowK[TR];
-  uint4 *const lq = smem, *const lg = smem + kTile;
+  static_assert(TR % 64 == 0 || TR == 32, "rows voted on 64 at a time");
+  constexpr int S = stages_of(32 * kTile);
+  __shared__ uint4 smem[2 * S * kTile > kMerge ? 2 * S * kTile : kMerge];   // S stages of q and do
+  __shared__ __attribute__((aligned(16))) float rowL[2][TR], rowD[2][TR];
+  constexpr bool PARK = parked<T, DH>();
+  __shared__ uint4 own[PARK ? 4 * NS * 64 : 1];
   int bh, tile, split;
   decode(a, bh, tile, split);
   tile = a.tiles - 1 - tile;   // early keys are the long ones here
@@ -466,9 +670,15 @@ __global__ __launch_bounds__(256) void k_attn_dkv(AttnArgs a) {
   const int b = bh / a.Hkv, hk = bh % a.Hkv;
   const int k0 = tile * 32 * WN, key = k0 + wn * 32 + (lane & 31);
   const bool kok = key < a.Tk && !(a.mask && a.mask[(long)b * a.Tk + min(key, a.Tk - 1)]);
-  frag kf[NS], vf[NS];
+  frag kf[NS];
+  Own<T, DH, PARK> vf;
   load_rows<T, DH>(kf, kok ? static_cast<const T*>(a.k) + b * a.sk.b + hk * a.sk.h + (long)key * a.sk.t : nullptr, a.D, lane);
-  load_rows<T, DH>(vf, kok ? static_cast<const T*>(a.v) + b * a.sv.b + hk * a.sv.h + (long)key * a.sv.t : nullptr, a.D, lane);
+  {
+    frag v[NS];
+    load_rows<T, DH>(v, kok ? static_cast<const T*>(a.v) + b * a.sv.b + hk * a.sv.h + (long)key * a.sv.t : nullptr, a.D, lane);
+    vf.park(own, wave, lane);
+    vf.set(v);
+  }
   f32x16 dk[MT], dv[MT];
 #pragma unroll
   for (int m = 0; m < MT; ++m) dk[m] = dv[m] = f32x16{0};
@@ -476,55 +686,77 @@ __global__ __launch_bounds__(256) void k_attn_dkv(AttnArgs a) {
 
   const T* const Q = static_cast<const T*>(a.q) + b * a.sq.b + (long)hk * a.G * a.sq.h;
   const T* const Go = static_cast<const T*>(a.go) + b * a.sgo.b + (long)hk * a.G * a.sgo.h;
-  const int steps = __syncthreads_or(kok) ? (a.R + TR - 1) / TR : 0;   // all keys masked: zeros
-  auto needed = [&](int st) {   // some row of the step sees some key of this tile
-    if (!a.causal) return true;
-    const int ra = st * TR, rb = min(ra + TR, a.R) - 1;
-    const int t = ra / a.Tq == rb / a.Tq ? rb % a.Tq : a.Tq - 1;
-    return t + a.off >= k0;
-  };
+  // a step: TR rows of one query head (none crosses heads); causal: heads' first rows that see key k0
+  const int per = (a.Tq + TR - 1) / TR;
+  const int steps = __syncthreads_or(kok) ? a.G * per : 0;   // all keys masked: zeros
+  auto needed = [&](int st) { return !a.causal || min((st % per + 1) * TR, a.Tq) - 1 + a.off >= k0; };
   auto after = [&](int st) {
     do st += a.splits; while (st < steps && !needed(st));
     return st;
   };
-  Stage<T, DH, TR> sq, sg;
-  float nL = 0.f, nD = 0.f;
-  int nK = 0;
+  // a step's lse and delta, one step ahead of its rows: lane l holds those of rows l, l + 64; a row that sees nothing (or does not exist) enters as zeros,
+  // whatever stands in it
+  constexpr int NB = (TR + 63) / 64;
+  float nL[NB], nD[NB];
+  unsigned long long live[NB];
+  auto stats = [&](int st) {
+    const int g = st / per, t0 = (st - g * per) * TR;
+    const long at = (long)bh * a.R + (long)g * a.Tq;
+#pragma unroll
+    for (int i = 0; i < NB; ++i) {
+      const int row = 64 * i + lane, t = t0 + row;
+      const bool in = row < TR && t < a.Tq;
+      nL[i] = in ? a.lse[at + t] : -inf();
+      nD[i] = in ? a.delta[at + t] : 0.f;
+    }
+  };
+  int stage = 0;
   auto fetch = [&](int st) {
-    const int r0 = st * TR;
-    auto where = [&](int row, const Str& s, const T* base) -> const T* {
-      const int r = r0 + row;
-      if (r >= a.R) return nullptr;
-      if (a.lse[(long)bh * a.R + r] == -inf()) return nullptr;   // a row that sees nothing: whatever stands in it stays out
-      const int g = a.G == 1 ? 0 : r / a.Tq;
-      return base + g * s.h + (long)(r - g * a.Tq) * s.t;
-    };
-    sq.load([&](int row, int) { return where(row, a.sq, Q); }, a.D);
-    sg.load([&](int row, int) { return where(row, a.sgo, Go); }, a.D);
-    if (threadIdx.x < TR) {
-      const int r = r0 + threadIdx.x;
-      nL = inf();
-      nD = 0.f;
-      nK = -1;
-      if (r < a.R) {
-        const float lse = a.lse[(long)bh * a.R + r];
-        nL = lse == -inf() ? inf() : lse * kLog2e;
-        nD = a.delta[(long)bh * a.R + r];
-        nK = a.causal ? (a.G == 1 ? r : r % a.Tq) + a.off : INT_MAX;
+    const int g = st / per, t0 = (st - g * per) * TR;
+    const T* const q = Q + g * a.sq.h + (long)t0 * a.sq.t;
+    const T* const go = Go + g * a.sgo.h + (long)t0 * a.sgo.t;
+#pragma unroll
+    for (int i = 0; i < NB; ++i) {
+      live[i] = __ballot(nL[i] != -inf());
+      if (wave == i && (TR >= 64 || lane < TR)) {
+        rowL[stage][64 * i + lane] = nL[i] == -inf() ? inf() : nL[i] * kLog2e;
+        rowD[stage][64 * i + lane] = nL[i] == -inf() ? 0.f : nD[i];
       }
     }
+    auto has = [&](int row) { return (live[NB == 1 ? 0 : row >> 6] >> (row & 63)) & 1; };
+    uint4* const to = smem + stage * 2 * kTile;
+    Fill<T, DH, TR>::issue(to, [&](int row) { return has(row) ? q + (long)row * a.sq.t : nullptr; }, a.D);
+    Fill<T, DH, TR>::issue(to + kTile, [&](int row) { return has(row) ? go + (long)row * a.sgo.t : nullptr; }, a.D);
   };
   int st = split;
   if (st < steps && !needed(st)) st = after(st);
-  if (st < steps) fetch(st);
+  int nx = st < steps ? after(st) : steps;
+  if (st < steps) {
+    stats(st);
+    if (S == 2) {
+      fetch(st);
+      if (nx < steps) stats(nx);
+    }
+  }
   while (st < steps) {
-    __syncthreads();
-    sq.store(lq);
-    sg.store(lg);
-    if (threadIdx.x < TR) { rowL[threadIdx.x] = nL; rowD[threadIdx.x] = nD; rowK[threadIdx.x] = nK; }
-    __syncthreads();
-    st = after(st);
-    if (st < steps) fetch(st);
+    if constexpr (S == 1) {
+      __syncthreads();
+      fetch(st);
+      if (nx < steps) stats(nx);
+    }
+    landed();
+    const uint4 *const lq = smem + stage * 2 * kTile, *const lg = lq + kTile;
+    const float *const rL = rowL[stage], *const rD = rowD[stage];
+    const int here = (st % per) * TR;
+    if constexpr (S == 2) stage ^= 1;
+    st = nx;
+    if (st < steps) {
+      nx = after(st);
+      if constexpr (S == 2) {
+        fetch(st);
+        if (nx < steps) stats(nx);
+      }
+    }
 #pragma unroll
     for (int u = 0; u < NU; ++u) {
       f32x16 s = {0}, dp = {0};
@@ -532,20 +764,18 @@ __global__ __launch_bounds__(256) void k_attn_dkv(AttnArgs a) {
 #pragma unroll
       for (int i = 0; i < NS; ++i) {
         s = Elem<T>::mma(Tl::row(lq, rr + (lane & 31), 2 * i + hi), kf[i], s);
-        dp = Elem<T>::mma(Tl::row(lg, rr + (lane & 31), 2 * i + hi), vf[i], dp);
+        dp = Elem<T>::mma(Tl::row(lg, rr + (lane & 31), 2 * i + hi), vf.get(i), dp);
       }
       f32x16 p;
 #pragma unroll
       for (int q = 0; q < 4; ++q) {
         const int rq = rr + 8 * q + 4 * hi;
-        const f32x4 L = *reinterpret_cast<const f32x4*>(rowL + rq), dl = *reinterpret_cast<const f32x4*>(rowD + rq);
-        typedef int i32x4 __attribute__((ext_vector_type(4)));
-        const i32x4 kl = *reinterpret_cast<const i32x4*>(rowK + rq);
+        const f32x4 L = *reinterpret_cast<const f32x4*>(rL + rq), dl = *reinterpret_cast<const f32x4*>(rD + rq);
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           const int e = 4 * q + i;
           float x = exp2_(__builtin_fmaf(s[e], a.c, PShift<T>::log2 - L[i]));
-          if (a.causal) x = key <= kl[i] ? x : 0.f;
+          if (a.causal) x = key <= here + a.off + rq + i ? x : 0.f;
           p[e] = x;
           s[e] = x * PShift<T>::back * (dp[e] - dl[i]);
         }
@@ -583,7 +813,7 @@ __global__ __launch_bounds__(256) void k_attn_dkv(AttnArgs a) {
     float* const red = reinterpret_cast<float*>(smem);
 #pragma unroll
     for (int which = 0; which < 2; ++which) {
-      __syncthreads();
+      landed();
       put_rows<DH>(red + wr * 32 * DH, which ? dv : dk, which ? fv : f, lane);
       __syncthreads();
       for (int i = threadIdx.x; i < 32 * (DH / 4); i += 256) {
@@ -603,16 +833,17 @@ __global__ __launch_bounds__(256) void k_attn_dkv(AttnArgs a) {
 namespace {
 
 // How a pass is cut.  Four waves x 32 rows share every staged tile where that alone gives two workgroups per CU; below, 32-row workgroups
-// whose waves share the keys; and while even those leave CUs empty the other axis is split over workgroups and joined.
+// whose waves share the keys; and while even those leave CUs empty the other axis is split over workgroups and joined.  512 workgroups are resident;
+// causal tiles differ in length by up to all of it, and twice as many workgroups as are resident, long ones first, even that out.
 struct Plan { int narrow, tiles, splits; };   // narrow: 32 rows per workgroup
-Plan plan_of(int nb, int rows, int across) {
+Plan plan_of(int nb, int rows, int across, bool causal) {
   Plan p;
   const long n32 = (long)nb * ((rows + 31) / 32);
   p.narrow = n32 <= 512;
   p.tiles = p.narrow ? (rows + 31) / 32 : (rows + 127) / 128;
-  const long base = (long)nb * p.tiles;
+  const long base = std::max<long>(1, (long)nb * p.tiles), want = causal ? 1024 : 512;
   const int steps = p.narrow ? (across + 127) / 128 : (across + 63) / 64;
-  long s = base >= 256 ? 1 : (512 + base - 1) / (base > 0 ? base : 1);
+  long s = base > want * 3 / 4 ? 1 : (want + base / 2) / base;
   s = std::min<long>(s, steps / 2);
   p.splits = (int)std::max<long>(1, std::min<long>(s, 64));
   return p;
@@ -651,7 +882,10 @@ Str str_of(const fdx_bht* t) { return t ? Str{(long)t->b, (long)t->h, (long)t->t
 size_t fwd_floats(const fdx_attn_desc* d, Plan p) {
   return p.splits > 1 ? (size_t)d->batch * d->heads * d->q_len * p.splits * (d->head_dim + 2) : 0;
 }
-size_t dq_floats(const fdx_attn_desc* d, Plan p) { return p.splits > 1 ? (size_t)d->batch * d->heads * d->q_len * p.splits * d->head_dim : 0; }
+size_t dq_floats(const fdx_attn_desc* d, Plan p) {
+  const size_t row = d->dtype == DT_F32 ? d->head_dim : 2 * d->head_dim + 1;
+  return p.splits > 1 ? (size_t)d->batch * d->heads * d->q_len * p.splits * row : 0;
+}
 size_t dkv_floats(const fdx_attn_desc* d, Plan p) { return p.splits > 1 ? (size_t)2 * d->batch * d->kv_heads * d->k_len * p.splits * d->head_dim : 0; }
 size_t delta_floats(const fdx_attn_desc* d) { return ((size_t)d->batch * d->heads * d->q_len + 3) / 4 * 4; }
 
@@ -691,13 +925,13 @@ template <typename T, int DH> struct RunBwd {
     if (a.R > 0) {
       a.tiles = pq.tiles; a.splits = pq.splits;
       const unsigned grid = (unsigned)((long)a.B * a.Hkv * pq.tiles * pq.splits);
-      e = pq.narrow ? launch(k_attn_dq<T, DH, 1, 32>, grid, 256, a, s) : launch(k_attn_dq<T, DH, 4, 64>, grid, 256, a, s);
-      if (e == hipSuccess && pq.splits > 1) e = join(a, part, a.dq, a.sdq, a.R, a.Tq, s);
+      e = pq.narrow ? launch(k_attn_dq<T, DH, 1, 32>, grid, 256, a, s) : launch(k_attn_dq<T, DH, 4, DQ_KT(T, DH)>, grid, 256, a, s);
+      if (e == hipSuccess && pq.splits > 1) e = launch(k_attn_join_dq<T>, (unsigned)(((long)a.B * a.Hkv * a.R + 3) / 4), 256, a, s);
     }
     if (e == hipSuccess && a.Tk > 0) {   // (reuses the partial sums' memory: ordered by the stream)
       a.tiles = pk.tiles; a.splits = pk.splits;
       const unsigned grid = (unsigned)((long)a.B * a.Hkv * pk.tiles * pk.splits);
-      e = pk.narrow ? launch(k_attn_dkv<T, DH, 1, 32>, grid, 256, a, s) : launch(k_attn_dkv<T, DH, 4, 64>, grid, 256, a, s);
+      e = pk.narrow ? launch(k_attn_dkv<T, DH, 1, 32>, grid, 256, a, s) : launch(k_attn_dkv<T, DH, 4, DKV_RT(T, DH)>, grid, 256, a, s);
       if (e == hipSuccess && pk.splits > 1) {
         const size_t half = (size_t)a.B * a.Hkv * a.splits * a.Tk * a.D;
         e = join(a, part, a.dk, a.sdk, a.Tk, a.Tk, s);
@@ -714,7 +948,7 @@ extern "C" int fdx_attn_forward_workspace(const fdx_attn_desc* d, size_t* bytes)
   if (const char* why = check(d)) return fail(nullptr, FDX_E_ARG, "fdx_attn_forward_workspace: %s", why);
   if (!bytes) return fail(nullptr, FDX_E_ARG, "fdx_attn_forward_workspace: null size pointer");
   const int rows = d->heads / d->kv_heads * d->q_len;
-  *bytes = fwd_floats(d, plan_of(d->batch * d->kv_heads, rows, d->k_len)) * sizeof(float);
+  *bytes = fwd_floats(d, plan_of(d->batch * d->kv_heads, rows, d->k_len, d->causal)) * sizeof(float);
   return FDX_OK;
 }
 
@@ -722,7 +956,7 @@ extern "C" int fdx_attn_backward_workspace(const fdx_attn_desc* d, size_t* bytes
   if (const char* why = check(d)) return fail(nullptr, FDX_E_ARG, "fdx_attn_backward_workspace: %s", why);
   if (!bytes) return fail(nullptr, FDX_E_ARG, "fdx_attn_backward_workspace: null size pointer");
   const int rows = d->heads / d->kv_heads * d->q_len, nb = d->batch * d->kv_heads;
-  *bytes = (delta_floats(d) + std::max(dq_floats(d, plan_of(nb, rows, d->k_len)), dkv_floats(d, plan_of(nb, d->k_len, rows)))) * sizeof(float);
+  *bytes = (delta_floats(d) + std::max(dq_floats(d, plan_of(nb, rows, d->k_len, d->causal)), dkv_floats(d, plan_of(nb, d->k_len, rows, d->causal)))) * sizeof(float);
   return FDX_OK;
 }
 
@@ -737,7 +971,7 @@ extern "C" int fdx_attn_forward(fdx_handle h, const fdx_attn_desc* d, const fdx_
     if (const char* why = check(d, x.t, x.need)) return fail(h, FDX_E_ARG, "fdx_attn_forward: %s", why);
   if (!lse) return fail(h, FDX_E_ARG, "fdx_attn_forward: null lse");
   AttnArgs a = args_of(d);
-  const Plan p = plan_of(a.B * a.Hkv, a.R, a.Tk);
+  const Plan p = plan_of(a.B * a.Hkv, a.R, a.Tk, a.causal);
   if (bytes < fwd_floats(d, p) * sizeof(float) || (p.splits > 1 && !workspace))
     return fail(h, FDX_E_ARG, "fdx_attn_forward: workspace of %zu bytes, %zu needed", bytes, fwd_floats(d, p) * sizeof(float));
   a.q = q->data; a.k = k ? k->data : nullptr; a.v = v ? v->data : nullptr; a.o = out->data;
@@ -761,7 +995,7 @@ extern "C" int fdx_attn_backward(fdx_handle h, const fdx_attn_desc* d, const fdx
     if (const char* why = check(d, x.t, x.need)) return fail(h, FDX_E_ARG, "fdx_attn_backward: %s", why);
   if (rows && !lse) return fail(h, FDX_E_ARG, "fdx_attn_backward: null lse");
   AttnArgs a = args_of(d);
-  const Plan pq = plan_of(a.B * a.Hkv, a.R, a.Tk), pk = plan_of(a.B * a.Hkv, a.Tk, a.R);
+  const Plan pq = plan_of(a.B * a.Hkv, a.R, a.Tk, a.causal), pk = plan_of(a.B * a.Hkv, a.Tk, a.R, a.causal);
   const size_t need = (delta_floats(d) + std::max(dq_floats(d, pq), dkv_floats(d, pk))) * sizeof(float);
   if (bytes < need || (need && !workspace)) return fail(h, FDX_E_ARG, "fdx_attn_backward: workspace of %zu bytes, %zu needed", bytes, need);
   const auto data = [](const fdx_bht* t) { return t ? t->data : nullptr; };
