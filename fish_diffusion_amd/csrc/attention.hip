@@ -21,13 +21,6 @@
 
 using namespace fdx;
 
-#ifndef FWD_W
-#define FWD_W(T, DH) 1
-#define DQ_W(T, DH) 1
-#define DKV_W(T, DH) 1
-#define DKV_RT(T, DH) 64
-#define DQ_KT(T, DH) 64
-#endif
 namespace {
 
 struct Str { long b, h, t; };
@@ -40,6 +33,10 @@ struct AttnArgs {
   int B, H, Hkv, G, Tq, Tk, D, R, off, causal, splits, tiles;
   float c, scale;        // c = scale * log2(e)
 };
+
+// Two waves on a SIMD (256 registers each): the exponentials of one run under the matrix instructions of the other.  fp32 at head size 128 holds 128
+// accumulators and as many operands and stays at one.  (bf16, head size 128, 2 x 16 x 4096 causal forward: 353 us with one wave, 238 with two.)
+template <typename T, int DH> constexpr int waves_of() { return sizeof(T) == 4 && DH == 128 ? 1 : 2; }
 
 constexpr float kLn2 = 0.69314718055994530942f, kLog2e = 1.44269504088896340736f;
 __device__ inline float inf() { return __builtin_inff(); }
@@ -140,12 +137,14 @@ template <typename T, int DH, bool PARK> struct Own {
   static constexpr int NS = DH / Elem<T>::KS;
   frag f[PARK ? 1 : NS];
   uint4* at;
-  __device__ inline void park(uint4* lds, int wave, int lane) { at = lds + wave * NS * 64 + lane; }
-  __device__ inline void set(const frag* v) {
+  // waves that share rows share their place: one of them writes it, before a barrier
+  __device__ inline void set(const frag* v, uint4* lds, int place, bool write, int lane) {
+    at = lds + place * NS * 64 + lane;
 #pragma unroll
     for (int s = 0; s < NS; ++s) {
-      if constexpr (PARK) at[s * 64] = __builtin_bit_cast(uint4, v[s]);
-      else f[s] = v[s];
+      if constexpr (PARK) {
+        if (write) at[s * 64] = __builtin_bit_cast(uint4, v[s]);
+      } else f[s] = v[s];
     }
   }
   __device__ inline frag get(int s) const {
@@ -196,13 +195,13 @@ template <> struct PShift<f16_t> { static constexpr float log2 = 14.f, back = 0x
 // WQ waves take 32 rows each, the other factor of the 4 waves (WK) shares those rows and takes KT keys each of every step; their
 // (max, sum, O) meet in LDS at the end.  Online softmax: running maximum m of the raw scores, P = exp2(c s - c m).
 template <typename T, int DH, int WQ, int KT>
-__global__ __launch_bounds__(256, FWD_W(T, DH)) void k_attn_fwd(AttnArgs a) {
+__global__ __launch_bounds__(256, (waves_of<T, DH>())) void k_attn_fwd(AttnArgs a) {
   typedef Tile<T, DH> Tl;
   typedef typename Elem<T>::frag frag;
   constexpr int KS = Elem<T>::KS, WK = 4 / WQ, TK = KT * WK, NS = DH / KS, MT = DH / 32, NU = KT / 32, NP = 32 / KS;
   constexpr int kTile = TK * Tl::CPR, kMerge = WK > 1 ? WK * 32 * DH / 4 : 0;   // in 16-byte units
   constexpr int S = stages_of(32 * kTile);
-  __shared__ uint4 smem[2 * S * kTile > kMerge ? 2 * S * kTile : kMerge];       // S stages of K and V
+  __shared__ __attribute__((aligned(1024))) uint4 smem[2 * S * kTile > kMerge ? 2 * S * kTile : kMerge];       // S stages of K and V
   __shared__ float ml[2][4][32];
   int bh, tile, split;
   decode(a, bh, tile, split);
@@ -223,6 +222,7 @@ __global__ __launch_bounds__(256, FWD_W(T, DH)) void k_attn_fwd(AttnArgs a) {
 
   RowBits<TK> rb;
   int stage = 0;
+  const unsigned row0 = lds_of(smem) + Tl::row_base(lane) + wk * KT * Tl::CPR * 16, col0 = lds_of(smem) + Tl::col_base(lane) + wk * KT * Tl::CPR * 16;
   auto fetch = [&](int st) {   // (masked rows enter as zeros: 0 * NaN never happens)
     const int k0 = st * TK;
     uint4* const to = smem + stage * 2 * kTile;
@@ -244,7 +244,8 @@ __global__ __launch_bounds__(256, FWD_W(T, DH)) void k_attn_fwd(AttnArgs a) {
       rb.load(mask, (st + a.splits) * TK, a.Tk, lane);
     }
     landed();
-    const uint4 *const lk = smem + stage * 2 * kTile, *const lv = lk + kTile;
+    const unsigned row = opaque(row0 + stage * 2 * kTile * 16), col = opaque(col0 + stage * 2 * kTile * 16);   // K; V: kTile rows' bytes behind
+    constexpr int V0 = TK;
     unsigned long long bits = rb.bits[wk * KT / 64];
     if constexpr (KT == 32) bits = (bits >> (wk * KT % 64)) & 0xffffffffull;
     if constexpr (S == 2) stage ^= 1;
@@ -261,10 +262,10 @@ __global__ __launch_bounds__(256, FWD_W(T, DH)) void k_attn_fwd(AttnArgs a) {
     for (int u = 0; u < NU; ++u) {
       s[u] = f32x16{0};
 #pragma unroll
-      for (int i = 0; i < NS; ++i) s[u] = Elem<T>::mma(Tl::row(lk, wk * KT + 32 * u + (lane & 31), 2 * i + hi), qf[i], s[u]);
+      for (int i = 0; i < NS; ++i) s[u] = Elem<T>::mma(Tl::row(row, 32 * u, i), qf[i], s[u]);
     }
     const int rel = lim - (st * TK + wk * KT);   // last visible key of this lane's row, relative
-    const unsigned long long full = KT == 64 ? ~0ull : (1ull << KT) - 1;
+    constexpr unsigned long long full = ~0ull >> (64 - KT);
     if (!__all(bits == full && rel >= KT - 1)) {
       unsigned long long ok = bits & (rel >= 63 ? ~0ull : rel < 0 ? 0ull : (2ull << rel) - 1);
 #pragma unroll
@@ -300,7 +301,7 @@ __global__ __launch_bounds__(256, FWD_W(T, DH)) void k_attn_fwd(AttnArgs a) {
       for (int p = 0; p < NP; ++p) {
         const frag pf = acc_frag<T>(s[u], p);
 #pragma unroll
-        for (int m = 0; m < MT; ++m) acc[m] = Elem<T>::mma(Tl::col(lv, wk * KT + 32 * u + KS * p, m, lane), pf, acc[m]);
+        for (int m = 0; m < MT; ++m) acc[m] = Elem<T>::mma(Tl::col(col, V0 + 32 * u + KS * p, m), pf, acc[m]);
       }
   }
   l += other_half(l);
@@ -405,17 +406,17 @@ struct RunScale {
 // 16-bit types: delta = do.o sees o as it was rounded, off by d.  P(dP - delta) sums to 0 over a row, so the sum r of what was computed IS d, up to
 // fp32: dq = scale (sum dS k - r sum P k), at the price of one more product whose operand is in place, and the dk / dv pass gets delta + r.
 template <typename T, int DH, int WQ, int KT>
-__global__ __launch_bounds__(256, DQ_W(T, DH)) void k_attn_dq(AttnArgs a) {
+__global__ __launch_bounds__(256, (waves_of<T, DH>())) void k_attn_dq(AttnArgs a) {
   typedef Tile<T, DH> Tl;
   typedef typename Elem<T>::frag frag;
   constexpr bool kScaled = DtOf<T>::v == DT_F16, kMend = sizeof(T) == 2;
   constexpr int KS = Elem<T>::KS, WK = 4 / WQ, TK = KT * WK, NS = DH / KS, MT = DH / 32, NU = KT / 32, NP = 32 / KS;
   constexpr int kTile = TK * Tl::CPR, kMerge = WK > 1 ? WK * 32 * DH / 4 : 0;
   constexpr int S = stages_of(32 * kTile);
-  __shared__ uint4 smem[2 * S * kTile > kMerge ? 2 * S * kTile : kMerge];
+  __shared__ __attribute__((aligned(1024))) uint4 smem[2 * S * kTile > kMerge ? 2 * S * kTile : kMerge];
   __shared__ float rest[4][32];
   constexpr bool PARK = parked<T, DH>();
-  __shared__ uint4 own[PARK ? 4 * NS * 64 : 1];
+  __shared__ uint4 own[PARK ? WQ * NS * 64 : 1];
   int bh, tile, split;
   decode(a, bh, tile, split);
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wq = wave / WK, wk = wave % WK, hi = lane >> 5;
@@ -429,6 +430,7 @@ __global__ __launch_bounds__(256, DQ_W(T, DH)) void k_attn_dq(AttnArgs a) {
   const uint8_t* const mask = a.mask ? a.mask + (long)b * a.Tk : nullptr;
   RowBits<TK> rb;
   int stage = 0;
+  const unsigned row0 = lds_of(smem) + Tl::row_base(lane) + wk * KT * Tl::CPR * 16, col0 = lds_of(smem) + Tl::col_base(lane) + wk * KT * Tl::CPR * 16;
   auto fetch = [&](int st) {
     const int k0 = st * TK;
     uint4* const to = smem + stage * 2 * kTile;
@@ -459,8 +461,7 @@ __global__ __launch_bounds__(256, DQ_W(T, DH)) void k_attn_dq(AttnArgs a) {
       for (int j = 0; j < Elem<T>::VEC; ++j) delta = __builtin_fmaf((float)go[s][j], (float)of[s][j], delta);
     delta += other_half(delta);
     if (empty) delta = 0.f;   // (whatever stands in do there)
-    gf.park(own, wave, lane);
-    gf.set(go);
+    gf.set(go, own, wq, wk == 0, lane);
   }
   const float L = empty ? inf() : lse * kLog2e;   // exp2(x - inf) = 0
   f32x16 acc[MT], pk[kMend ? MT : 1];
@@ -480,7 +481,8 @@ __global__ __launch_bounds__(256, DQ_W(T, DH)) void k_attn_dq(AttnArgs a) {
       rb.load(mask, (st + a.splits) * TK, a.Tk, lane);
     }
     landed();
-    const uint4 *const lk = smem + stage * 2 * kTile, *const lv = lk + kTile;
+    const unsigned row = opaque(row0 + stage * 2 * kTile * 16), col = opaque(col0 + stage * 2 * kTile * 16);   // K; V: kTile rows' bytes behind
+    constexpr int V0 = TK;
     unsigned long long bits = rb.bits[wk * KT / 64];
     if constexpr (KT == 32) bits = (bits >> (wk * KT % 64)) & 0xffffffffull;
     if constexpr (S == 2) stage ^= 1;
@@ -493,17 +495,16 @@ __global__ __launch_bounds__(256, DQ_W(T, DH)) void k_attn_dq(AttnArgs a) {
     }
     if (bits == 0) continue;
     const int rel = lim - (st * TK + wk * KT);
-    const unsigned long long full = KT == 64 ? ~0ull : (1ull << KT) - 1;
+    constexpr unsigned long long full = ~0ull >> (64 - KT);
     const bool whole = __all(bits == full && rel >= KT - 1 && !empty);
     const unsigned long long ok = empty ? 0ull : bits & (rel >= 63 ? ~0ull : rel < 0 ? 0ull : (2ull << rel) - 1);
 #pragma unroll
     for (int u = 0; u < NU; ++u) {
       f32x16 s = {0}, dp = {0};
-      const int kr = wk * KT + 32 * u;
 #pragma unroll
       for (int i = 0; i < NS; ++i) {
-        s = Elem<T>::mma(Tl::row(lk, kr + (lane & 31), 2 * i + hi), qf[i], s);
-        dp = Elem<T>::mma(Tl::row(lv, kr + (lane & 31), 2 * i + hi), gf.get(i), dp);
+        s = Elem<T>::mma(Tl::row(row, 32 * u, i), qf[i], s);
+        dp = Elem<T>::mma(Tl::row(row, V0 + 32 * u, i), gf.get(i), dp);
       }
 #pragma unroll
       for (int e = 0; e < 16; ++e) s[e] = exp2_(__builtin_fmaf(s[e], a.c, PShift<T>::log2 - L));
@@ -530,7 +531,7 @@ __global__ __launch_bounds__(256, DQ_W(T, DH)) void k_attn_dq(AttnArgs a) {
         if constexpr (kMend) pf = acc_frag<T>(s, p);
 #pragma unroll
         for (int m = 0; m < MT; ++m) {
-          const frag kf = Tl::col(lk, kr + KS * p, m, lane);
+          const frag kf = Tl::col(col, 32 * u + KS * p, m);
           acc[m] = Elem<T>::mma(kf, df, acc[m]);
           if constexpr (kMend) pk[m] = Elem<T>::mma(kf, pf, pk[m]);
         }
@@ -651,7 +652,7 @@ template <typename T> __global__ __launch_bounds__(256) void k_attn_join_sum(Joi
 
 // dk, dv: WN waves own 32 keys each, the other factor (WR) shares those keys and takes RT rows each of every step
 template <typename T, int DH, int WN, int RT>
-__global__ __launch_bounds__(256, DKV_W(T, DH)) void k_attn_dkv(AttnArgs a) {
+__global__ __launch_bounds__(256, (waves_of<T, DH>())) void k_attn_dkv(AttnArgs a) {
   typedef Tile<T, DH> Tl;
   typedef typename Elem<T>::frag frag;
   constexpr bool kScaled = DtOf<T>::v == DT_F16;
@@ -659,10 +660,10 @@ __global__ __launch_bounds__(256, DKV_W(T, DH)) void k_attn_dkv(AttnArgs a) {
   constexpr int kTile = TR * Tl::CPR, kMerge = WR > 1 ? WR * 32 * DH / 4 : 0;
   static_assert(TR % 64 == 0 || TR == 32, "rows voted on 64 at a time");
   constexpr int S = stages_of(32 * kTile);
-  __shared__ uint4 smem[2 * S * kTile > kMerge ? 2 * S * kTile : kMerge];   // S stages of q and do
+  __shared__ __attribute__((aligned(1024))) uint4 smem[2 * S * kTile > kMerge ? 2 * S * kTile : kMerge];   // S stages of q and do
   __shared__ __attribute__((aligned(16))) float rowL[2][TR], rowD[2][TR];
   constexpr bool PARK = parked<T, DH>();
-  __shared__ uint4 own[PARK ? 4 * NS * 64 : 1];
+  __shared__ uint4 own[PARK ? WN * NS * 64 : 1];
   int bh, tile, split;
   decode(a, bh, tile, split);
   tile = a.tiles - 1 - tile;   // early keys are the long ones here
@@ -676,8 +677,7 @@ __global__ __launch_bounds__(256, DKV_W(T, DH)) void k_attn_dkv(AttnArgs a) {
   {
     frag v[NS];
     load_rows<T, DH>(v, kok ? static_cast<const T*>(a.v) + b * a.sv.b + hk * a.sv.h + (long)key * a.sv.t : nullptr, a.D, lane);
-    vf.park(own, wave, lane);
-    vf.set(v);
+    vf.set(v, own, wn, wr == 0, lane);
   }
   f32x16 dk[MT], dv[MT];
 #pragma unroll
@@ -711,6 +711,7 @@ __global__ __launch_bounds__(256, DKV_W(T, DH)) void k_attn_dkv(AttnArgs a) {
     }
   };
   int stage = 0;
+  const unsigned row0 = lds_of(smem) + Tl::row_base(lane) + wr * RT * Tl::CPR * 16, col0 = lds_of(smem) + Tl::col_base(lane) + wr * RT * Tl::CPR * 16;
   auto fetch = [&](int st) {
     const int g = st / per, t0 = (st - g * per) * TR;
     const T* const q = Q + g * a.sq.h + (long)t0 * a.sq.t;
@@ -745,7 +746,7 @@ __global__ __launch_bounds__(256, DKV_W(T, DH)) void k_attn_dkv(AttnArgs a) {
       if (nx < steps) stats(nx);
     }
     landed();
-    const uint4 *const lq = smem + stage * 2 * kTile, *const lg = lq + kTile;
+    const unsigned row = opaque(row0 + stage * 2 * kTile * 16), col = opaque(col0 + stage * 2 * kTile * 16);   // q; do: TR rows behind
     const float *const rL = rowL[stage], *const rD = rowD[stage];
     const int here = (st % per) * TR;
     if constexpr (S == 2) stage ^= 1;
@@ -763,8 +764,8 @@ __global__ __launch_bounds__(256, DKV_W(T, DH)) void k_attn_dkv(AttnArgs a) {
       const int rr = wr * RT + 32 * u;
 #pragma unroll
       for (int i = 0; i < NS; ++i) {
-        s = Elem<T>::mma(Tl::row(lq, rr + (lane & 31), 2 * i + hi), kf[i], s);
-        dp = Elem<T>::mma(Tl::row(lg, rr + (lane & 31), 2 * i + hi), vf.get(i), dp);
+        s = Elem<T>::mma(Tl::row(row, 32 * u, i), kf[i], s);
+        dp = Elem<T>::mma(Tl::row(row, TR + 32 * u, i), vf.get(i), dp);
       }
       f32x16 p;
 #pragma unroll
@@ -786,8 +787,8 @@ __global__ __launch_bounds__(256, DKV_W(T, DH)) void k_attn_dkv(AttnArgs a) {
         const frag pf = acc_frag<T>(p, i), df = acc_frag<T>(s, i);
 #pragma unroll
         for (int m = 0; m < MT; ++m) {
-          dv[m] = Elem<T>::mma(Tl::col(lg, rr + KS * i, m, lane), pf, dv[m]);
-          dk[m] = Elem<T>::mma(Tl::col(lq, rr + KS * i, m, lane), df, dk[m]);
+          dv[m] = Elem<T>::mma(Tl::col(col, TR + 32 * u + KS * i, m), pf, dv[m]);
+          dk[m] = Elem<T>::mma(Tl::col(col, 32 * u + KS * i, m), df, dk[m]);
         }
       }
     }
@@ -925,13 +926,13 @@ template <typename T, int DH> struct RunBwd {
     if (a.R > 0) {
       a.tiles = pq.tiles; a.splits = pq.splits;
       const unsigned grid = (unsigned)((long)a.B * a.Hkv * pq.tiles * pq.splits);
-      e = pq.narrow ? launch(k_attn_dq<T, DH, 1, 32>, grid, 256, a, s) : launch(k_attn_dq<T, DH, 4, DQ_KT(T, DH)>, grid, 256, a, s);
+      e = pq.narrow ? launch(k_attn_dq<T, DH, 1, 32>, grid, 256, a, s) : launch(k_attn_dq<T, DH, 4, (DH * sizeof(T) >= 256 ? 32 : 64)>, grid, 256, a, s);
       if (e == hipSuccess && pq.splits > 1) e = launch(k_attn_join_dq<T>, (unsigned)(((long)a.B * a.Hkv * a.R + 3) / 4), 256, a, s);
     }
     if (e == hipSuccess && a.Tk > 0) {   // (reuses the partial sums' memory: ordered by the stream)
       a.tiles = pk.tiles; a.splits = pk.splits;
       const unsigned grid = (unsigned)((long)a.B * a.Hkv * pk.tiles * pk.splits);
-      e = pk.narrow ? launch(k_attn_dkv<T, DH, 1, 32>, grid, 256, a, s) : launch(k_attn_dkv<T, DH, 4, DKV_RT(T, DH)>, grid, 256, a, s);
+      e = pk.narrow ? launch(k_attn_dkv<T, DH, 1, 32>, grid, 256, a, s) : launch(k_attn_dkv<T, DH, 4, (DH * sizeof(T) >= 256 ? 32 : 64)>, grid, 256, a, s);
       if (e == hipSuccess && pk.splits > 1) {
         const size_t half = (size_t)a.B * a.Hkv * a.splits * a.Tk * a.D;
         e = join(a, part, a.dk, a.sdk, a.Tk, a.Tk, s);

@@ -185,7 +185,7 @@ __global__ __launch_bounds__(256) void k_linear8_wgrad(WgradArgs a) {
   typedef Tile<bf16_t, 128> Tl;
   typedef Elem<bf16_t>::frag frag;
   constexpr int P = Planes<T>::n, KT = 32;
-  __shared__ uint4 ly[P][KT * 16], lx[KT * 16];
+  __shared__ __attribute__((aligned(1024))) uint4 ly[P][KT * 16], lx[KT * 16];
   __shared__ float lb[16][128];
   const int per = a.to * a.ti, split = blockIdx.x / per, j = blockIdx.x % per, o0 = j / a.ti * 128, i0 = j % a.ti * 128;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wo = wave >> 1, wi = wave & 1;
@@ -198,6 +198,7 @@ __global__ __launch_bounds__(256) void k_linear8_wgrad(WgradArgs a) {
   for (int m = 0; m < 2; ++m)
 #pragma unroll
     for (int n = 0; n < 2; ++n) acc[m][n] = f32x16{0};
+  const unsigned coly = lds_of(ly) + (Tl::col_base(lane) ^ (128 * wo)), colx = lds_of(lx) + (Tl::col_base(lane) ^ (128 * wi));
   const long nb = (long)split * a.rows, ne = min(a.N, nb + a.rows);
   float y[2][8], x[2][8];
   auto fetch = [&](long n0) {
@@ -248,12 +249,12 @@ __global__ __launch_bounds__(256) void k_linear8_wgrad(WgradArgs a) {
     for (int ks = 0; ks < KT / 16; ++ks) {
       frag b[2];
 #pragma unroll
-      for (int n = 0; n < 2; ++n) b[n] = Tl::col(lx, 16 * ks, 2 * wi + n, lane);
+      for (int n = 0; n < 2; ++n) b[n] = Tl::col(colx, 16 * ks, n);
 #pragma unroll
       for (int p = P - 1; p >= 0; --p)   // small parts first
 #pragma unroll
         for (int m = 0; m < 2; ++m) {
-          const frag f = Tl::col(ly[p], 16 * ks, 2 * wo + m, lane);
+          const frag f = Tl::col(coly, p * KT + 16 * ks, m);
 #pragma unroll
           for (int n = 0; n < 2; ++n) acc[m][n] = Elem<bf16_t>::mma(f, b[n], acc[m][n]);
         }

@@ -17,6 +17,8 @@ typedef _Float16 f16_t;
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef short s16x8 __attribute__((ext_vector_type(8)));
+typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
 
 template <typename T> struct Elem;
 template <> struct Elem<float> {
@@ -57,35 +59,43 @@ template <typename T, int DH> struct Tile {
     }
   }
   static __device__ inline int at(int r, int c) { return r * CPR + (c ^ swz(r)); }   // in chunks
-  static __device__ inline frag row(const uint4* t, int r, int c) {
-    return __builtin_bit_cast(frag, t[at(r, c)]);
+
+  // LDS byte addresses.  x() takes row bits 0 ... 3 only and a row is a power of two of bytes, so a lane's address is ONE number xored with constants
+  // (which chunk) plus constants (which rows): two registers per lane address every fragment of a tile.
+  template <typename V> static __device__ inline V lds(unsigned at) { return *reinterpret_cast<__attribute__((address_space(3))) const V*>((size_t)at); }
+  // row fragments: rows r0 + (lane & 31), r0 a multiple of 16; chunk 2 * i + (lane >> 5)
+  static __device__ inline unsigned row_base(int lane) { return (unsigned)at(lane & 31, lane >> 5) * 16; }
+  static __device__ inline frag row(unsigned base, int r0, int i) { return __builtin_bit_cast(frag, lds<u32x4>((base ^ (32 * i)) + r0 * CPR * 16)); }
+  // column fragments: rows r0 + (column order above) of columns 32 * m + (lane & 31); r0 a multiple of KS
+  static __device__ inline unsigned col_base(int lane) {
+    if constexpr (sizeof(T) == 4) return (unsigned)at(4 * (lane >> 5), (lane & 31) >> 2) * 16 + (lane & 3) * 4;
+    else return (unsigned)at(4 * (lane >> 5) + ((lane & 15) >> 2), 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1)) * 16 + (lane & 1) * 8;
   }
-  // rows r0 + (column order above) of columns 32 * m + (lane & 31); r0 a multiple of KS
-  static __device__ inline frag col(const uint4* t, int r0, int m, int lane) {
-    const int hi = lane >> 5;
+  static __device__ inline frag col(unsigned base, int r0, int m) {
     if constexpr (sizeof(T) == 4) {
       frag f;
-      const int c = lane & 31;
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        const int r = r0 + 4 * hi + j;
-        f[j] = reinterpret_cast<const float*>(t)[at(r, 8 * m + (c >> 2)) * 4 + (c & 3)];
+        const int x = (CPR == 8 ? j >> 1 : j) ^ (r0 & 8 ? 4 : 0);   // x(r0 + 4 * (lane >> 5) + j) ^ x(4 * (lane >> 5))
+        f[j] = lds<float>((base ^ (128 * m) ^ (16 * x)) + (r0 + j) * CPR * 16);
       }
       return f;
     } else {
       // ds_read_b64_tr_b16: the 16 lanes of a group read 4 rows x 16 columns (lane i: row i >> 2, columns 4 * (i & 3) ...), lane i receives column i
-      const int c = 4 * m + 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1);
-      const int ra = r0 + 4 * hi + ((lane & 15) >> 2), rb = ra + 8;
       typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
-      const char* p = reinterpret_cast<const char*>(t);
-      const s16x4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(p + at(ra, c) * 16 + (lane & 1) * 8));
-      const s16x4 b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(p + at(rb, c) * 16 + (lane & 1) * 8));
-      typedef short s16x8 __attribute__((ext_vector_type(8)));
-      const s16x8 v = __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
-      return __builtin_bit_cast(frag, v);
+      const s16x4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(size_t)((base ^ (64 * m)) + r0 * CPR * 16));
+      const s16x4 b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(size_t)((base ^ (64 * m) ^ 32) + (r0 + 8) * CPR * 16));   // x(r + 8) = x(r) ^ 2
+      return __builtin_bit_cast(frag, __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7));
     }
   }
 };
+
+__device__ inline unsigned lds_of(const void* p) { return (unsigned)(size_t)(__attribute__((address_space(3))) const char*)p; }
+// a value the compiler must not precompute from: keeps what is derived from it inside the loop instead of in registers across it
+__device__ inline unsigned opaque(unsigned x) {
+  asm volatile("" : "+v"(x));
+  return x;
+}
 
 // accumulator rows of k-step s (KS rows) as an operand; one rounding to T (half a step of T relative) where T is 16 bits
 template <typename T> __device__ inline typename Elem<T>::frag acc_frag(const f32x16& v, int s) {
