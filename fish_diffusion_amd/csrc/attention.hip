@@ -61,40 +61,9 @@ __device__ inline int key_end(const AttnArgs& a, int r0, int r1) {
   return max(0, min(a.Tk, t + a.off + 1));
 }
 
-__device__ __attribute__((aligned(16))) unsigned g_zero[4];   // where rows that do not exist are read
-
-// TK rows of DH elements from memory straight to LDS (global_load_lds_dwordx4: a wave-instruction lands 64 chunks in a row at a wave-uniform address, so
-// the tile's swizzle is applied to the SOURCE address).  No staging registers: that is what lets two workgroups share a CU.  The loads are counted by
-// the wait in front of the barrier that publishes the tile (landed()); written as asm because with the builtin in flight the compiler waits for every
-// LDS read.  A load has no register output, so nothing can overwrite what is in flight.
-template <typename T, int DH, int TK> struct Fill {
-  typedef Tile<T, DH> Tl;
-  static constexpr int N = TK * Tl::CPR / 256, RPI = 64 / Tl::CPR > 0 ? 64 / Tl::CPR : 1;   // wave-instructions per wave, rows each covers
-  static_assert(N * 256 == TK * Tl::CPR && 64 % Tl::CPR == 0, "whole rows per instruction");
-  template <typename F> static __device__ inline void issue(uint4* lds, F&& src, int D) {   // src(row): its address, or null (zeros)
-    const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), lane = threadIdx.x & 63;
-    const unsigned base = (unsigned)(size_t)(__attribute__((address_space(3))) uint4*)lds;
-#pragma unroll
-    for (int i = 0; i < N; ++i) {
-      const int row = (i * 4 + wave) * RPI + lane / Tl::CPR, c = (lane % Tl::CPR) ^ Tl::swz(row);
-      const T* p = src(row);
-      const void* from = p && c * Elem<T>::VEC < D ? static_cast<const void*>(p + c * Elem<T>::VEC) : g_zero;
-      const unsigned to = base + (unsigned)(i * 4 + wave) * 1024u;
-      unsigned keep;
-      asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off\n\ts_mov_b32 m0, %0"
-                   : "=&s"(keep) : "v"(from), "s"(to) : "memory");
-    }
-  }
-};
 // stages of a tile pair of `bytes`: two (a step's loads fly while the one before is computed) where two workgroups still fit on a CU, else one (the
 // other workgroup's products cover the loads)
 constexpr int stages_of(int bytes) { return 2 * bytes <= 80 * 1024 ? 2 : 1; }
-
-// every wave's loads into LDS have landed, and every wave is done with the tile before
-__device__ inline void landed() {
-  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-  __syncthreads();
-}
 
 // which of a step's TK rows exist and are not masked, in every wave: loaded one step before it is needed
 template <int TK> struct RowBits {

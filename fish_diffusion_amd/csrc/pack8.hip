@@ -162,14 +162,16 @@ template <typename T, bool GRAD> __global__ __launch_bounds__(256) void k_unpack
 }
 
 // ---------------------------------------------------------------------------------------------------------------- weight gradient
-// A workgroup computes a 128 x 128 tile of dW over its share of the rows n: 32 rows of dy (in bf16 planes) and of x8 (decoded) at a time in LDS, both
-// read as column fragments by transposing reads, 4 waves of 64 x 64.  Rows are shared out over `splits` workgroups whose fp32 partial tiles a second
-// launch joins in order.  db is added up by the threads that stage dy in the first column of tiles.
+// A workgroup computes a tile of dW over its share of the rows n, 64 * MO output by 128 input channels, in four waves of (32 * MO) x 64.  KT rows of dy
+// (in bf16 planes) and of x8 (decoded) stand in LDS, two stages, both read as column fragments by transposing reads: MO + 2 fragments feed 2 * MO matrix
+// instructions, so at MO = 4 the LDS delivers 3/4 of what it can while they run.  bf16 dy goes straight to LDS; the wider types pass registers to be split.
+// Rows are shared out over `splits` workgroups (an XCD takes whole shares: dy and x8 stay in its L2 for all tiles) whose fp32 partial tiles a second
+// launch joins in order.  db is summed from what is staged, each tile column taking every ti-th step.
 struct WgradArgs {
   const void* dy;
   const int8_t* codes;
   const uint8_t* exps;
-  float *part, *part_b;   // [splits][O][I], [splits][O]
+  float *part, *part_b;   // [splits][O][I], [splits][ti][O]
   long N, rows;           // rows per split: a multiple of 32
   int O, I, G, to, ti, splits, bias, vec_dy, vec_x;
 };
@@ -179,115 +181,245 @@ template <> struct Planes<bf16_t> { static constexpr int n = 1; };
 template <> struct Planes<f16_t> { static constexpr int n = 2; };
 
 __device__ inline unsigned hi_bits(float x) { return __builtin_bit_cast(unsigned, x) & 0xffff0000u; }
+__device__ inline unsigned pair(unsigned lo, unsigned up) { return __builtin_amdgcn_perm(up, lo, 0x07060302); }   // the upper halves of two words
 
-template <typename T>
-__global__ __launch_bounds__(256) void k_linear8_wgrad(WgradArgs a) {
+// 8 codes as 8 bf16 numbers (exact)
+__device__ inline uint4 decode8(uint2 c, float scale) {
+  uint4 w;
+  unsigned* const wp = &w.x;
+#pragma unroll
+  for (int q = 0; q < 4; ++q) {
+    const unsigned v = q < 2 ? c.x : c.y;
+    const float f0 = (float)(signed char)(v >> (16 * (q & 1))) * scale, f1 = (float)(signed char)(v >> (16 * (q & 1) + 8)) * scale;
+    wp[q] = pair(__builtin_bit_cast(unsigned, f0), __builtin_bit_cast(unsigned, f1));
+  }
+  return w;
+}
+
+template <typename T, int MO>
+__global__ __launch_bounds__(256, 2) void k_linear8_wgrad(WgradArgs a) {
   typedef Tile<bf16_t, 128> Tl;
   typedef Elem<bf16_t>::frag frag;
-  constexpr int P = Planes<T>::n, KT = 32;
-  __shared__ __attribute__((aligned(1024))) uint4 ly[P][KT * 16], lx[KT * 16];
-  __shared__ float lb[16][128];
-  const int per = a.to * a.ti, split = blockIdx.x / per, j = blockIdx.x % per, o0 = j / a.ti * 128, i0 = j % a.ti * 128;
+  constexpr int P = Planes<T>::n, KT = P == 1 ? 32 : 16, NO = MO / 2;   // NO: 128-channel tiles of dy
+  constexpr int kY = KT * 16, kX = KT * 16, kStage = P * NO * kY + kX;   // in 16-byte units
+  __shared__ __attribute__((aligned(1024))) uint4 smem[2 * kStage];
+  const int per = a.to * a.ti;
+  int split, j;
+  if (a.splits % 8 == 0) { split = (blockIdx.x & 7) + 8 * ((blockIdx.x >> 3) / per); j = (blockIdx.x >> 3) % per; }
+  else { split = blockIdx.x / per; j = blockIdx.x % per; }
+  const int jo = j / a.ti, ji = j % a.ti, o0 = jo * 128 * NO, i0 = ji * 128;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wo = wave >> 1, wi = wave & 1;
-  const int chunk = threadIdx.x & 15, srow = threadIdx.x >> 4;   // staging: 8 columns of rows srow, srow + 16
-  const int oc = o0 + 8 * chunk, on = a.O - oc, ic = i0 + 8 * chunk, in = a.I - ic;
-  const bool want_b = a.bias && i0 == 0;
+  // staging of x: 8 columns of XR rows; of dy (through registers): 8 columns of YR rows
+  constexpr int XR = KT / 16, YC = 16 * NO, YR = KT * YC / 256;
+  const int xc = threadIdx.x & 15, xr = threadIdx.x >> 4, yc = threadIdx.x % YC, yr = threadIdx.x / YC;
+  const int ic = i0 + 8 * xc, in = a.I - ic, oc = o0 + 8 * yc, on = a.O - oc;
   float db[8] = {0, 0, 0, 0, 0, 0, 0, 0};
-  f32x16 acc[2][2];
+  f32x16 acc[MO][2];
 #pragma unroll
-  for (int m = 0; m < 2; ++m)
+  for (int m = 0; m < MO; ++m)
 #pragma unroll
     for (int n = 0; n < 2; ++n) acc[m][n] = f32x16{0};
-  const unsigned coly = lds_of(ly) + (Tl::col_base(lane) ^ (128 * wo)), colx = lds_of(lx) + (Tl::col_base(lane) ^ (128 * wi));
   const long nb = (long)split * a.rows, ne = min(a.N, nb + a.rows);
-  float y[2][8], x[2][8];
-  auto fetch = [&](long n0) {
+  // wave wo's channels: MO == 4: its own 128-channel tile, MO == 2: half of the one
+  const unsigned coly = lds_of(smem) + (Tl::col_base(lane) ^ (MO == 2 ? 128 * wo : 0)) + (MO == 4 ? wo * P * kY * 16 : 0);
+  const unsigned colx = lds_of(smem) + P * NO * kY * 16 + (Tl::col_base(lane) ^ (128 * wi));
+
+  uint2 xcode[XR];
+  int xexp[XR];
+  float y[P == 1 ? 1 : YR][8];
+  auto load_x = [&](long n0) {
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const long n = n0 + srow + 16 * h;
-      const bool ok = n < ne;
-      load8<T>(static_cast<const T*>(a.dy) + n * a.O + oc, ok ? on : 0, a.vec_dy, y[h]);
-      if (ok && in > 0) load_codes(a.codes + n * a.I + ic, in, a.vec_x, pow2_of(a.exps[n * a.G + (ic >> 5)]), x[h]);
-      else {
+    for (int h = 0; h < XR; ++h) {
+      const long n = n0 + xr + 16 * h;
+      const bool ok = n < ne && in > 0;
+      const int8_t* const p = a.codes + n * a.I + ic;
+      xcode[h] = uint2{0, 0};
+      xexp[h] = ok ? a.exps[n * a.G + (ic >> 5)] : 0;
+      if (ok) {
+        if (a.vec_x) xcode[h] = *reinterpret_cast<const uint2*>(p);
+        else {
 #pragma unroll
-        for (int q = 0; q < 8; ++q) x[h][q] = 0.f;
+          for (int q = 0; q < 8; ++q)
+            if (q < in) (q < 4 ? xcode[h].x : xcode[h].y) |= (unsigned)(uint8_t)p[q] << (8 * (q & 3));
+        }
       }
     }
   };
-  if (nb < ne) fetch(nb);
-  for (long n0 = nb; n0 < ne; n0 += KT) {
-    __syncthreads();
+  auto load_y = [&](long n0) {   // P > 1, or rows that cannot be read 16 bytes at a time
+    if constexpr (P > 1) {
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const int at = Tl::at(srow + 16 * h, chunk);
-      if (want_b) {
-#pragma unroll
-        for (int q = 0; q < 8; ++q) db[q] += y[h][q];
+      for (int h = 0; h < YR; ++h) {
+        const long n = n0 + yr + (256 / YC) * h;
+        load8<T>(static_cast<const T*>(a.dy) + n * a.O + oc, n < ne ? on : 0, a.vec_dy, y[h]);
       }
-#pragma unroll
-      for (int p = 0; p < P; ++p) {
-        uint4 w;
-        unsigned* const wp = &w.x;
-#pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          const unsigned lo = hi_bits(y[h][2 * q]), up = hi_bits(y[h][2 * q + 1]);
-          wp[q] = (lo >> 16) | up;
-          y[h][2 * q] -= __builtin_bit_cast(float, lo);   // exact: the remaining low bits
-          y[h][2 * q + 1] -= __builtin_bit_cast(float, up);
-        }
-        ly[p][at] = w;
-      }
-      uint4 w;
-      unsigned* const wp = &w.x;
-#pragma unroll
-      for (int q = 0; q < 4; ++q) wp[q] = (hi_bits(x[h][2 * q]) >> 16) | hi_bits(x[h][2 * q + 1]);
-      lx[at] = w;
     }
-    __syncthreads();
-    if (n0 + KT < ne) fetch(n0 + KT);
+  };
+  // brings dy's rows of a step (and, from registers, x's) into a stage
+  auto fill = [&](long n0, int stage, bool count) {
+    uint4* const to = smem + stage * kStage;
+    if constexpr (P == 1) {
+      if (a.vec_dy) {
+#pragma unroll
+        for (int h = 0; h < NO; ++h)
+          Fill<bf16_t, 128, KT>::issue(to + h * kY, [&](int row) { return n0 + row < ne ? static_cast<const bf16_t*>(a.dy) + (n0 + row) * a.O + o0 + 128 * h : nullptr; },
+                                       a.O - o0 - 128 * h);
+      } else {
+#pragma unroll
+        for (int h = 0; h < YR; ++h) {
+          const int row = yr + (256 / YC) * h;
+          float v[8];
+          load8<T>(static_cast<const T*>(a.dy) + (n0 + row) * a.O + oc, n0 + row < ne ? on : 0, false, v);
+          uint4 w;
+          unsigned* const wp = &w.x;
+#pragma unroll
+          for (int q = 0; q < 4; ++q) wp[q] = pair(__builtin_bit_cast(unsigned, v[2 * q]), __builtin_bit_cast(unsigned, v[2 * q + 1]));
+          to[(yc >> 4) * kY + Tl::at(row, yc & 15)] = w;
+        }
+      }
+    } else {
+#pragma unroll
+      for (int h = 0; h < YR; ++h) {
+        if (count) {
+#pragma unroll
+          for (int q = 0; q < 8; ++q) db[q] += y[h][q];
+        }
+        const int at = (yc >> 4) * P * kY + Tl::at(yr + (256 / YC) * h, yc & 15);
+#pragma unroll
+        for (int p = 0; p < P; ++p) {
+          uint4 w;
+          unsigned* const wp = &w.x;
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            float &lo = y[h][2 * q], &up = y[h][2 * q + 1];
+            wp[q] = pair(__builtin_bit_cast(unsigned, lo), __builtin_bit_cast(unsigned, up));
+            if (p + 1 < P) {   // exact: the bits below
+              lo -= __builtin_bit_cast(float, hi_bits(lo));
+              up -= __builtin_bit_cast(float, hi_bits(up));
+            }
+          }
+          to[at + p * kY] = w;
+        }
+      }
+    }
+#pragma unroll
+    for (int h = 0; h < XR; ++h) to[P * NO * kY + Tl::at(xr + 16 * h, xc)] = decode8(xcode[h], pow2_of(xexp[h]));
+  };
+  auto mine = [&](long n0) { return a.bias && (n0 - nb) / KT % a.ti == ji; };
+  int stage = 0;
+  if (nb < ne) {
+    load_y(nb);
+    load_x(nb);
+    fill(nb, 0, mine(nb));
+    if (nb + KT < ne) { load_y(nb + KT); load_x(nb + KT); }
+  }
+  for (long n0 = nb; n0 < ne; n0 += KT) {
+    landed();
+    const unsigned cy = opaque(coly + stage * kStage * 16), cx = opaque(colx + stage * kStage * 16);
+    if (n0 + KT < ne) {
+      fill(n0 + KT, stage ^ 1, mine(n0 + KT));
+      if (n0 + 2 * KT < ne) { load_y(n0 + 2 * KT); load_x(n0 + 2 * KT); }
+    }
+    if constexpr (P == 1) {
+      if (mine(n0)) {
+        const uint4* const t = smem + stage * kStage + (yc >> 4) * kY;
+#pragma unroll
+        for (int h = 0; h < YR; ++h) {
+          const frag v = __builtin_bit_cast(frag, t[Tl::at(yr + (256 / YC) * h, yc & 15)]);
+#pragma unroll
+          for (int q = 0; q < 8; ++q) db[q] += (float)v[q];
+        }
+      }
+    }
 #pragma unroll
     for (int ks = 0; ks < KT / 16; ++ks) {
       frag b[2];
 #pragma unroll
-      for (int n = 0; n < 2; ++n) b[n] = Tl::col(colx, 16 * ks, n);
+      for (int n = 0; n < 2; ++n) b[n] = Tl::col(cx, 16 * ks, n);
 #pragma unroll
       for (int p = P - 1; p >= 0; --p)   // small parts first
 #pragma unroll
-        for (int m = 0; m < 2; ++m) {
-          const frag f = Tl::col(coly, p * KT + 16 * ks, m);
+        for (int m = 0; m < MO; ++m) {
+          const frag f = Tl::col(cy, p * KT + 16 * ks, m);
 #pragma unroll
           for (int n = 0; n < 2; ++n) acc[m][n] = Elem<bf16_t>::mma(f, b[n], acc[m][n]);
         }
     }
+    stage ^= 1;
   }
   float* const out = a.part + (long)split * a.O * a.I;
 #pragma unroll
-  for (int m = 0; m < 2; ++m)
+  for (int m = 0; m < MO; ++m)
 #pragma unroll
     for (int n = 0; n < 2; ++n)
 #pragma unroll
       for (int e = 0; e < 16; ++e) {
-        const int o = o0 + wo * 64 + m * 32 + 8 * (e >> 2) + 4 * (lane >> 5) + (e & 3), i = i0 + wi * 64 + n * 32 + (lane & 31);
+        const int o = o0 + wo * 32 * MO + m * 32 + 8 * (e >> 2) + 4 * (lane >> 5) + (e & 3), i = i0 + wi * 64 + n * 32 + (lane & 31);
         if (o < a.O && i < a.I) out[(long)o * a.I + i] = acc[m][n][e];
       }
-  if (want_b) {   // (uniform over the workgroup)
+  if (a.bias) {
+    float* const lb = reinterpret_cast<float*>(smem);   // [256 / YC][8 * YC]
+    landed();
 #pragma unroll
-    for (int q = 0; q < 8; ++q) lb[srow][8 * chunk + q] = db[q];
+    for (int q = 0; q < 8; ++q) lb[yr * 8 * YC + 8 * yc + q] = db[q];
     __syncthreads();
-    if (threadIdx.x < 128 && o0 + (int)threadIdx.x < a.O) {
+    if ((int)threadIdx.x < 8 * YC && o0 + (int)threadIdx.x < a.O) {
       float s = 0.f;
-      for (int r = 0; r < 16; ++r) s += lb[r][threadIdx.x];
-      a.part_b[(long)split * a.O + o0 + threadIdx.x] = s;
+      for (int r = 0; r < 256 / YC; ++r) s += lb[r * 8 * YC + threadIdx.x];
+      a.part_b[((long)split * a.ti + ji) * a.O + o0 + threadIdx.x] = s;
     }
   }
 }
 
-struct Join8Args { const float* part; void* out; long n; int splits; };
+// The partial tiles joined in their order, four elements a thread with eight loads in flight; behind them db: 32 channels a workgroup, every thread sums an
+// eighth of the rows.
+struct Join8Args { const float *part, *part_b; void *dw, *db; long n; int splits, O, rows_b, main, vec; };
 template <typename T> __global__ __launch_bounds__(256) void k_join8(Join8Args a) {
-  for (long i = (long)blockIdx.x * 256 + threadIdx.x; i < a.n; i += (long)gridDim.x * 256) {
-    float v = 0.f;
-    for (int s = 0; s < a.splits; ++s) v += a.part[s * a.n + i];
-    static_cast<T*>(a.out)[i] = (T)v;
+  __shared__ float red[8][32];
+  if ((int)blockIdx.x < a.main) {
+    const long i = ((long)blockIdx.x * 256 + threadIdx.x) * 4;
+    if (i >= a.n) return;
+    if (a.vec) {
+      f32x4 v = {0, 0, 0, 0};
+      const float* p = a.part + i;
+      int s = 0;
+      for (; s + 8 <= a.splits; s += 8) {
+        f32x4 t[8];
+#pragma unroll
+        for (int q = 0; q < 8; ++q) t[q] = *reinterpret_cast<const f32x4*>(p + (s + q) * a.n);
+#pragma unroll
+        for (int q = 0; q < 8; ++q) v += t[q];
+      }
+      for (; s < a.splits; ++s) v += *reinterpret_cast<const f32x4*>(p + s * a.n);
+      typedef T vt __attribute__((ext_vector_type(4)));
+      *reinterpret_cast<vt*>(static_cast<T*>(a.dw) + i) = vt{(T)v[0], (T)v[1], (T)v[2], (T)v[3]};
+    } else {
+      for (long j = i; j < min(i + 4, a.n); ++j) {
+        float v = 0.f;
+        for (int s = 0; s < a.splits; ++s) v += a.part[s * a.n + j];
+        static_cast<T*>(a.dw)[j] = (T)v;
+      }
+    }
+    return;
+  }
+  const int c = ((int)blockIdx.x - a.main) * 32 + (threadIdx.x & 31), g = threadIdx.x >> 5;
+  float v = 0.f;
+  if (c < a.O) {
+    int r = g;
+    for (; r + 7 * 8 < a.rows_b; r += 8 * 8) {
+      float t[8];
+#pragma unroll
+      for (int q = 0; q < 8; ++q) t[q] = a.part_b[(long)(r + 8 * q) * a.O + c];
+#pragma unroll
+      for (int q = 0; q < 8; ++q) v += t[q];
+    }
+    for (; r < a.rows_b; r += 8) v += a.part_b[(long)r * a.O + c];
+  }
+  red[g][threadIdx.x & 31] = v;
+  __syncthreads();
+  if (g == 0 && c < a.O) {
+#pragma unroll
+    for (int q = 1; q < 8; ++q) v += red[q][threadIdx.x & 31];
+    static_cast<T*>(a.db)[c] = (T)v;
   }
 }
 
@@ -318,22 +450,21 @@ template <typename T> struct KGelu { static auto get() { return k_pack8<T, true>
 template <typename T> struct KUnpack { static auto get() { return k_unpack8<T, false>; } };
 template <typename T> struct KGeluGrad { static auto get() { return k_unpack8<T, true>; } };
 
-// Rows are split until two workgroups stand on every CU, each of them with 256 rows at least: a shorter share costs more in partial tiles
-// (8 bytes per element of dW and share) than it gains.
-int wgrad_splits(long N, int O, int I) {
-  const long tiles = (long)((O + 127) / 128) * ((I + 127) / 128);
-  const long s = std::min<long>((512 + tiles - 1) / tiles, N / 256);
-  return (int)std::max<long>(1, std::min<long>(s, 64));
+// 256-channel tiles where they fit the output channels as well as 128-channel ones do.  Rows are split until two workgroups stand on every CU, each of
+// them with 256 rows at least: a shorter share costs more in partial tiles (8 bytes per element of dW and share) than it gains.
+struct Cut8 { int wide, to, ti, splits; };
+Cut8 wgrad_cut(long N, int O, int I) {
+  Cut8 c;
+  c.wide = O > 128 && ((O + 127) / 128) % 2 == 0;
+  c.to = (O + (c.wide ? 255 : 127)) / (c.wide ? 256 : 128);
+  c.ti = (I + 127) / 128;
+  const long tiles = (long)c.to * c.ti;
+  long s = std::min<long>((512 + tiles - 1) / tiles, N / 256);
+  if (s > 8) s = s / 8 * 8;
+  c.splits = (int)std::max<long>(1, std::min<long>(s, 64));
+  return c;
 }
-size_t wgrad_floats(long N, int O, int I) { return (size_t)wgrad_splits(N, O, I) * ((size_t)O * I + O); }
-
-template <typename T> hipError_t join8(const float* part, void* out, long n, int splits, hipStream_t s) {
-  Join8Args j{part, out, n, splits};
-  return launch(k_join8<T>, (unsigned)std::min<long>((n + 255) / 256, 4096), 256, j, s);
-}
-hipError_t join8(int dt, const float* part, void* out, long n, int splits, hipStream_t s) {
-  return dt == DT_F32 ? join8<float>(part, out, n, splits, s) : dt == DT_BF16 ? join8<bf16_t>(part, out, n, splits, s) : join8<f16_t>(part, out, n, splits, s);
-}
+size_t wgrad_floats(const Cut8& c, int O, int I) { return (size_t)c.splits * ((size_t)O * I + (size_t)c.ti * O); }
 
 }  // namespace
 
@@ -397,7 +528,7 @@ extern "C" int fdx_linear8_weight_grad_workspace(int dtype, long long rows, int 
   if (!why) why = check(dtype, rows, in_features);
   if (!why && !bytes) why = "null size pointer";
   if (why) return fail(nullptr, FDX_E_ARG, "fdx_linear8_weight_grad_workspace: %s", why);
-  *bytes = wgrad_floats(rows, out_features, in_features) * sizeof(float);
+  *bytes = wgrad_floats(wgrad_cut(rows, out_features, in_features), out_features, in_features) * sizeof(float);
   return FDX_OK;
 }
 
@@ -408,25 +539,30 @@ extern "C" int fdx_linear8_weight_grad(fdx_handle h, int dtype, const void* dy, 
   const char* why = check(dtype, rows, out_features);
   if (!why) why = check(grad_dtype, rows, in_features);
   const long tiles = (long)((out_features + 127) / 128) * ((in_features + 127) / 128);
-  if (!why && tiles > INT_MAX / 64) why = "too many tiles for one launch";
+  if (!why && (tiles > INT_MAX / 64 || (long)out_features * in_features / 1024 > INT_MAX / 2)) why = "too many tiles for one launch";
   if (!why && (!dw || (rows > 0 && (!dy || !codes || !exps)))) why = "null tensor";
   if (why) return fail(h, FDX_E_ARG, "fdx_linear8_weight_grad: %s", why);
-  const size_t need = wgrad_floats(rows, out_features, in_features) * sizeof(float);
+  const Cut8 c = wgrad_cut(rows, out_features, in_features);
+  const size_t need = wgrad_floats(c, out_features, in_features) * sizeof(float);
   if (bytes < need || !workspace) return fail(h, FDX_E_ARG, "fdx_linear8_weight_grad: workspace of %zu bytes, %zu needed", bytes, need);
   WgradArgs a{};
   a.dy = dy; a.codes = codes; a.exps = exps; a.N = rows; a.O = out_features; a.I = in_features; a.G = (in_features + 31) / 32;
-  a.to = (a.O + 127) / 128; a.ti = (a.I + 127) / 128; a.splits = wgrad_splits(rows, a.O, a.I); a.bias = db != nullptr;
+  a.to = c.to; a.ti = c.ti; a.splits = c.splits; a.bias = db != nullptr;
   a.rows = ((rows + a.splits - 1) / a.splits + 31) / 32 * 32;
   a.vec_dy = aligned({dy}, a.O, 16); a.vec_x = aligned({codes}, a.I, 8);
   a.part = static_cast<float*>(workspace);
   a.part_b = a.part + (size_t)a.splits * a.O * a.I;
   DeviceScope dev(h->device);
   FDX_HIP(h, dev.err);
-  const unsigned grid = (unsigned)(tiles * a.splits);
   hipStream_t s = as_stream(st);
-  FDX_HIP(h, dtype == DT_F32 ? launch(k_linear8_wgrad<float>, grid, 256, a, s) : dtype == DT_BF16 ? launch(k_linear8_wgrad<bf16_t>, grid, 256, a, s)
-                                                                                              : launch(k_linear8_wgrad<f16_t>, grid, 256, a, s));
-  FDX_HIP(h, join8(grad_dtype, a.part, dw, (long)a.O * a.I, a.splits, s));
-  if (db) FDX_HIP(h, join8(grad_dtype, a.part_b, db, a.O, a.splits, s));
+  const auto go = [&](auto narrow, auto wide) { return launch(c.wide ? wide : narrow, (unsigned)((long)c.to * c.ti * c.splits), 256, a, s); };
+  FDX_HIP(h, dtype == DT_F32 ? go(k_linear8_wgrad<float, 2>, k_linear8_wgrad<float, 4>) : dtype == DT_BF16 ? go(k_linear8_wgrad<bf16_t, 2>, k_linear8_wgrad<bf16_t, 4>)
+                                                                                              : go(k_linear8_wgrad<f16_t, 2>, k_linear8_wgrad<f16_t, 4>));
+  Join8Args j{a.part, a.part_b, dw, db, (long)a.O * a.I, a.splits, a.O, a.splits * a.ti, 0, 0};
+  j.vec = j.n % 4 == 0 && (reinterpret_cast<uintptr_t>(dw) & 15) == 0 && (reinterpret_cast<uintptr_t>(workspace) & 15) == 0;
+  j.main = (int)((j.n + 1023) / 1024);
+  const unsigned grid = (unsigned)j.main + (db ? (a.O + 31) / 32 : 0);
+  FDX_HIP(h, grad_dtype == DT_F32 ? launch(k_join8<float>, grid, 256, j, s) : grad_dtype == DT_BF16 ? launch(k_join8<bf16_t>, grid, 256, j, s)
+                                                                                                    : launch(k_join8<f16_t>, grid, 256, j, s));
   return FDX_OK;
 }
