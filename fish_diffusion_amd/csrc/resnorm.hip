@@ -195,7 +195,7 @@ __global__ __launch_bounds__((Row<T, VEC, IT, NW>::kThreads)) void k_resnorm_fwd
     }
 #pragma unroll
     for (int e = 0; e < E; ++e) x[e] = __builtin_fmaf(a.a, x[e], a.gate ? g[e] * n[e] : n[e]);
-    R::each(a.C, [&](int c, int e) { st<T, VEC>(static_cast<T*>(a.h) + o + c, x + e); });
+    if (a.h) R::each(a.C, [&](int c, int e) { st<T, VEC>(static_cast<T*>(a.h) + o + c, x + e); });
     if (a.has_pre) {
       R::stats(x, a, buf, turn, m1, r1);
 #pragma unroll
@@ -478,7 +478,7 @@ extern "C" int fdx_resnorm_forward(fdx_handle h, const fdx_resnorm_desc* d, cons
   if (!h) return fail(nullptr, FDX_E_ARG, "fdx_resnorm_forward: null handle");
   if (const char* why = check(d)) return fail(h, FDX_E_ARG, "fdx_resnorm_forward: %s", why);
   if (d->rows == 0) return FDX_OK;
-  if (!x || !block || !out_h || (pre_w && !out_y) || (d->gate_rows > 0) != (gate != nullptr) || (post_b && !post_w) || (pre_b && !pre_w) ||
+  if (!x || !block || (!out_h && !pre_w) || (pre_w && !out_y) || (d->gate_rows > 0) != (gate != nullptr) || (post_b && !post_w) || (pre_b && !pre_w) ||
       (reinterpret_cast<uintptr_t>(stats) & 15))
     return fail(h, FDX_E_ARG, "fdx_resnorm_forward: null tensor, or gate_rows / weights that do not fit the tensors given");
   NormArgs a = args_of(d);

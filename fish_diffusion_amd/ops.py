@@ -290,15 +290,18 @@ def _norm_args(x, block, gate, residual_scale, post_norm, pre_norm, kind, eps, w
     return desc, [_packed_rows(p) for p in params]
 
 
-def residual_norm_forward(x, block, gate=None, residual_scale=1.0, post_norm=None, pre_norm=None, kind="layer", eps=1e-5):
+def residual_norm_forward(x, block, gate=None, residual_scale=1.0, post_norm=None, pre_norm=None, kind="layer", eps=1e-5, need_h=True):
     """(h, y, stats): h = residual_scale * x + gate * post_norm(block), y = pre_norm(h) (None without one), stats for the backward pass.
 
     x, block [..., C], C up to 8192; post_norm / pre_norm = (weight, bias or None) of a LayerNorm (kind "layer") or RMSNorm ("rms") over the last
     dimension, or None; gate None, [C], x's own shape, or for x [B, T, C] one row per item: [B, C] or [B, 1, C].  Weights, biases and gate may be fp32
-    beside 16-bit x.  y is computed from h before h is rounded.  A post-norm block's x = norm(x + block) is pre_norm alone, its result y."""
+    beside 16-bit x.  y is computed from h before h is rounded.  A post-norm block's x = norm(x + block) is pre_norm alone with need_h=False: h is None and not
+    written."""
+    if not need_h and pre_norm is None:
+        raise ValueError("residual_norm: need_h=False without a pre_norm leaves no result")
     desc, (pw, pb, nw, nb) = _norm_args(x, block, gate, residual_scale, post_norm, pre_norm, kind, eps, "residual_norm")
     x, block, gate = _packed_rows(x), _packed_rows(block), _packed_rows(gate)
-    h_out = torch.empty_like(x)
+    h_out = torch.empty_like(x) if need_h else None
     y = torch.empty_like(x) if nw is not None else None
     stats = torch.empty((*x.shape[:-1], 4), dtype=torch.float32, device=x.device)
     if x.numel():
@@ -340,9 +343,9 @@ def residual_norm_backward(grad_h, grad_y, x, block, stats, gate=None, residual_
 
 class _ResidualNorm(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x, block, gate, post_w, post_b, pre_w, pre_b, residual_scale, kind, eps):
+    def forward(ctx, x, block, gate, post_w, post_b, pre_w, pre_b, residual_scale, kind, eps, need_h):
         post, pre = (None if w is None else (w, b) for w, b in ((post_w, post_b), (pre_w, pre_b)))
-        h, y, stats = residual_norm_forward(x, block, gate, residual_scale, post, pre, kind, eps)
+        h, y, stats = residual_norm_forward(x, block, gate, residual_scale, post, pre, kind, eps, need_h)
         ctx.save_for_backward(x, block, gate, post_w, post_b, pre_w, pre_b, stats)
         ctx.rest = (residual_scale, kind, eps)
         ctx.set_materialize_grads(False)
@@ -354,12 +357,12 @@ class _ResidualNorm(torch.autograd.Function):
         x, block, gate, post_w, post_b, pre_w, pre_b, stats = ctx.saved_tensors
         residual_scale, kind, eps = ctx.rest
         post, pre = (None if w is None else (w, b) for w, b in ((post_w, post_b), (pre_w, pre_b)))
-        return (*residual_norm_backward(grad_h, grad_y, x, block, stats, gate, residual_scale, post, pre, kind, eps), None, None, None)
+        return (*residual_norm_backward(grad_h, grad_y, x, block, stats, gate, residual_scale, post, pre, kind, eps), None, None, None, None)
 
 
-def residual_norm(x, block, gate=None, residual_scale=1.0, post_norm=None, pre_norm=None, kind="layer", eps=1e-5):
+def residual_norm(x, block, gate=None, residual_scale=1.0, post_norm=None, pre_norm=None, kind="layer", eps=1e-5, need_h=True):
     """Differentiable `residual_norm_forward`: returns (h, y)."""
-    return _apply(_ResidualNorm, x, block, gate, *(post_norm or (None, None)), *(pre_norm or (None, None)), residual_scale, kind, eps)
+    return _apply(_ResidualNorm, x, block, gate, *(post_norm or (None, None)), *(pre_norm or (None, None)), residual_scale, kind, eps, need_h)
 
 
 # ------------------------------------------------------------------------------------------------------------- activations in 8 bits

@@ -440,7 +440,7 @@ int fdx_attn_backward(fdx_handle h, const fdx_attn_desc* d, const fdx_bht* grad_
 
 /* The step between two blocks: n = post(block), h = residual_scale x + gate n, y = pre(h) with post / pre LayerNorm or RMSNorm (weights given), or
  * nothing (NULL weights; bias NULL: none).  All tensors dev, [rows][channels] contiguous; gate [rows / gate_rows][channels]: gate_rows = rows is one
- * gate per channel, rows of an item one per item, 1 one per element, 0 no gate (NULL).  stats: dev fp32 [rows][4] for the backward pass, or NULL. */
+ * gate per channel, rows of an item one per item, 1 one per element, 0 no gate (NULL).  stats: dev fp32 [rows][4] for the backward pass, or NULL.  out_h may be NULL where only y is wanted. */
 typedef struct fdx_resnorm_desc {
   int dtype, param_dtype, gate_dtype;   /* x, block, h, y and gradients; the norms' weights and biases; the gate: the latter two dtype or FDX_F32 */
   long long rows;

@@ -240,3 +240,18 @@ def test_refusals_on_the_device():
             fda.residual_norm_backward(*args, **kw)
     with pytest.raises(ValueError):
         fda.residual_norm_backward(gh, gy, x, block, stats)
+
+
+def test_only_the_normalised_result():
+    import fish_diffusion_amd as fda
+    x, block, gh, gy, kw = make(torch.float32, (2, 9, 48), "channel", False, True, "layer")
+    h, y, stats = fda.residual_norm_forward(x, block, **kw)
+    none, y2, stats2 = fda.residual_norm_forward(x, block, **kw, need_h=False)
+    assert none is None and torch.equal(y, y2) and torch.equal(stats, stats2)
+    lx = x.clone().requires_grad_()
+    h, y = fda.residual_norm(lx, block, **kw, need_h=False)
+    assert h is None
+    y.backward(gy)
+    assert torch.equal(lx.grad, fda.residual_norm_backward(None, gy, x, block, stats, **kw).dx)
+    with pytest.raises(ValueError):
+        fda.residual_norm(x, block, need_h=False)
