@@ -41,7 +41,17 @@ template <typename T, int DH> constexpr int waves_of() { return sizeof(T) == 4 &
 constexpr float kLn2 = 0.69314718055994530942f, kLog2e = 1.44269504088896340736f;
 __device__ inline float inf() { return __builtin_inff(); }
 __device__ inline float exp2_(float x) { return __builtin_amdgcn_exp2f(x); }
-__device__ inline float other_half(float x) { return __shfl_xor(x, 32, 64); }
+// of lane l and lane l ^ 32, in both: the swap exchanges the upper half of its first register with the lower half of its second one, so it needs two
+__device__ inline float half_max(float x) {
+  const auto r = __builtin_amdgcn_permlane32_swap(__builtin_bit_cast(unsigned, x), opaque(__builtin_bit_cast(unsigned, x)), false, false);
+  const unsigned lo = r[0], up = r[1];   // (bit_cast of a vector element as it stands reads element 0)
+  return fmaxf(__builtin_bit_cast(float, lo), __builtin_bit_cast(float, up));
+}
+__device__ inline float half_sum(float x) {
+  const auto r = __builtin_amdgcn_permlane32_swap(__builtin_bit_cast(unsigned, x), opaque(__builtin_bit_cast(unsigned, x)), false, false);
+  const unsigned lo = r[0], up = r[1];
+  return __builtin_bit_cast(float, lo) + __builtin_bit_cast(float, up);
+}
 
 // workgroup -> (batch and kv head, tile, split).  Workgroups go to the 8 XCDs in turn: where the heads divide, all tiles of a head run on one
 // XCD and find its K / V in that XCD's L2.  Late (causal: long) tiles start first.
@@ -82,6 +92,12 @@ template <int TK> struct RowBits {
     for (int i = 0; i < N; ++i) bits[i] = __ballot(m[i] == 0);
   }
   __device__ inline bool has(int row) const { return (bits[N == 1 ? 0 : row >> 6] >> (row & 63)) & 1; }
+  __device__ inline bool all() const {
+    unsigned long long o = ~0ull;
+#pragma unroll
+    for (int i = 0; i < N; ++i) o &= bits[i];
+    return o == (TK < 64 ? ~0ull >> (64 - TK) : ~0ull);
+  }
   __device__ inline bool any() const {
     unsigned long long o = 0;
 #pragma unroll
@@ -156,9 +172,10 @@ template <int DH> __device__ inline f32x4 sum_rows(const float* red, int row, in
   return v;
 }
 
-// fp16: probabilities are carried times 2^14 (so <= 2^14), which keeps those down to 2^-28 normal numbers; every sum has the same factor.
+// fp16: probabilities are carried times 2^11 (at most 2^15, with the slack of the forward's reference), which keeps those down to 2^-25 normal numbers;
+// every sum has the same factor.
 template <typename T> struct PShift { static constexpr float log2 = 0.f, back = 1.f; };
-template <> struct PShift<f16_t> { static constexpr float log2 = 14.f, back = 0x1p-14f; };
+template <> struct PShift<f16_t> { static constexpr float log2 = 11.f, back = 0x1p-11f; };
 
 // ---------------------------------------------------------------------------------------------------------------- forward
 // WQ waves take 32 rows each, the other factor of the 4 waves (WK) shares those rows and takes KT keys each of every step; their
@@ -187,16 +204,19 @@ __global__ __launch_bounds__(256, (waves_of<T, DH>())) void k_attn_fwd(AttnArgs 
   f32x16 acc[MT];
 #pragma unroll
   for (int m = 0; m < MT; ++m) acc[m] = f32x16{0};
-  float mx = -inf(), l = 0.f;
+  float mc = -inf(), l = 0.f;   // the row's reference, times c; its sum
+  constexpr float kSlack = DtOf<T>::v == DT_F16 ? 4.f : 8.f;
 
   RowBits<TK> rb;
   int stage = 0;
   const unsigned row0 = lds_of(smem) + Tl::row_base(lane) + wk * KT * Tl::CPR * 16, col0 = lds_of(smem) + Tl::col_base(lane) + wk * KT * Tl::CPR * 16;
   auto fetch = [&](int st) {   // (masked rows enter as zeros: 0 * NaN never happens)
-    const int k0 = st * TK;
+    const long k0 = (long)st * TK;
     uint4* const to = smem + stage * 2 * kTile;
-    Fill<T, DH, TK>::issue(to, [&](int row) { return rb.has(row) ? K + (long)(k0 + row) * a.sk.t : nullptr; }, a.D);
-    Fill<T, DH, TK>::issue(to + kTile, [&](int row) { return rb.has(row) ? V + (long)(k0 + row) * a.sv.t : nullptr; }, a.D);
+    const bool all = a.D == DH && rb.all();
+    const auto has = [&](int row) { return rb.has(row); };
+    Fill<T, DH, TK>::issue(to, K + k0 * a.sk.t, a.sk.t, a.D, all, has);
+    Fill<T, DH, TK>::issue(to + kTile, V + k0 * a.sv.t, a.sv.t, a.D, all, has);
   };
   if (split < steps) {
     rb.load(mask, split * TK, a.Tk, lane);
@@ -244,26 +264,32 @@ __global__ __launch_bounds__(256, (waves_of<T, DH>())) void k_attn_fwd(AttnArgs 
         for (int e = 0; e < 16; ++e) s[u][e] = (w >> (8 * (e >> 2) + (e & 3))) & 1 ? s[u][e] : -inf();
       }
     }
-    float mt = mx;
+    float mt = -inf();
 #pragma unroll
     for (int u = 0; u < NU; ++u)
 #pragma unroll
       for (int e = 0; e < 16; ++e) mt = fmaxf(mt, s[u][e]);
-    mt = fmaxf(mt, other_half(mt));
-    const float mc = mt == -inf() ? 0.f : mt * a.c;
-    const float alpha = exp2_(mx * a.c - mc);
-    mx = mt;
+    mt = half_max(mt) * a.c;
+    // The reference of a row moves only when a score passes it by kSlack (powers of two): nearly never behind the first tiles
+    const bool move = mt > mc + kSlack || (mc == -inf() && mt > -inf());
+    if (__any(move)) {
+      const float to = move ? mt : mc;
+      const float alpha = to == -inf() ? 1.f : exp2_(mc - to);
+      mc = to;
+      l *= alpha;
+#pragma unroll
+      for (int m = 0; m < MT; ++m) acc[m] *= alpha;
+    }
+    const float ref = PShift<T>::log2 - (mc == -inf() ? 0.f : mc);
     float sum = 0.f;
 #pragma unroll
     for (int u = 0; u < NU; ++u)
 #pragma unroll
       for (int e = 0; e < 16; ++e) {
-        s[u][e] = exp2_(__builtin_fmaf(s[u][e], a.c, PShift<T>::log2 - mc));
+        s[u][e] = exp2_(__builtin_fmaf(s[u][e], a.c, ref));
         sum += s[u][e];
       }
-    l = l * alpha + sum;
-#pragma unroll
-    for (int m = 0; m < MT; ++m) acc[m] *= alpha;
+    l += sum;
 #pragma unroll
     for (int u = 0; u < NU; ++u)
 #pragma unroll
@@ -273,8 +299,7 @@ __global__ __launch_bounds__(256, (waves_of<T, DH>())) void k_attn_fwd(AttnArgs 
         for (int m = 0; m < MT; ++m) acc[m] = Elem<T>::mma(Tl::col(col, V0 + 32 * u + KS * p, m), pf, acc[m]);
       }
   }
-  l += other_half(l);
-  float mc = mx * a.c;   // -inf: no key seen
+  l = half_sum(l);
 
   const long row_out = (long)bh * a.R + r;
   T* const O = static_cast<T*>(a.o) + b * a.so.b + (hk * a.G + g) * a.so.h + t * a.so.t;
@@ -359,7 +384,7 @@ struct RunScale {
     float top = 0.f;
 #pragma unroll
     for (int e = 0; e < 16; ++e) top = fmaxf(top, fabsf(ds[e]));
-    top = fmaxf(top, other_half(top));
+    top = half_max(top);
     const bool move = top * s > 0x1p15f;
     if (__any(move)) {
       const float n = move ? __builtin_ldexpf(1.f, 14 - (int)((__builtin_bit_cast(unsigned, top) >> 23) & 255) + 127) : s, f = n / s;
@@ -401,10 +426,12 @@ __global__ __launch_bounds__(256, (waves_of<T, DH>())) void k_attn_dq(AttnArgs a
   int stage = 0;
   const unsigned row0 = lds_of(smem) + Tl::row_base(lane) + wk * KT * Tl::CPR * 16, col0 = lds_of(smem) + Tl::col_base(lane) + wk * KT * Tl::CPR * 16;
   auto fetch = [&](int st) {
-    const int k0 = st * TK;
+    const long k0 = (long)st * TK;
     uint4* const to = smem + stage * 2 * kTile;
-    Fill<T, DH, TK>::issue(to, [&](int row) { return rb.has(row) ? K + (long)(k0 + row) * a.sk.t : nullptr; }, a.D);
-    Fill<T, DH, TK>::issue(to + kTile, [&](int row) { return rb.has(row) ? V + (long)(k0 + row) * a.sv.t : nullptr; }, a.D);
+    const bool all = a.D == DH && rb.all();
+    const auto has = [&](int row) { return rb.has(row); };
+    Fill<T, DH, TK>::issue(to, K + k0 * a.sk.t, a.sk.t, a.D, all, has);
+    Fill<T, DH, TK>::issue(to + kTile, V + k0 * a.sv.t, a.sv.t, a.D, all, has);
   };
   if (split < steps) {
     rb.load(mask, split * TK, a.Tk, lane);
@@ -428,7 +455,7 @@ __global__ __launch_bounds__(256, (waves_of<T, DH>())) void k_attn_dq(AttnArgs a
     for (int s = 0; s < NS; ++s)
 #pragma unroll
       for (int j = 0; j < Elem<T>::VEC; ++j) delta = __builtin_fmaf((float)go[s][j], (float)of[s][j], delta);
-    delta += other_half(delta);
+    delta = half_sum(delta);
     if (empty) delta = 0.f;   // (whatever stands in do there)
     gf.set(go, own, wq, wk == 0, lane);
   }
@@ -509,7 +536,7 @@ __global__ __launch_bounds__(256, (waves_of<T, DH>())) void k_attn_dq(AttnArgs a
   }
   float f = a.scale;
   if constexpr (kScaled) f /= rs.s;
-  if constexpr (kMend) left += other_half(left);
+  if constexpr (kMend) left = half_sum(left);
   const float fp = a.scale * PShift<T>::back;   // of pk
   const long prow = ((long)bh * a.splits + split) * a.R;
   float* const part_pk = a.part + (long)a.B * a.Hkv * a.splits * a.R * a.D;
@@ -695,8 +722,11 @@ __global__ __launch_bounds__(256, (waves_of<T, DH>())) void k_attn_dkv(AttnArgs 
     }
     auto has = [&](int row) { return (live[NB == 1 ? 0 : row >> 6] >> (row & 63)) & 1; };
     uint4* const to = smem + stage * 2 * kTile;
-    Fill<T, DH, TR>::issue(to, [&](int row) { return has(row) ? q + (long)row * a.sq.t : nullptr; }, a.D);
-    Fill<T, DH, TR>::issue(to + kTile, [&](int row) { return has(row) ? go + (long)row * a.sgo.t : nullptr; }, a.D);
+    bool all = a.D == DH;
+#pragma unroll
+    for (int i = 0; i < NB; ++i) all = all && live[i] == (TR < 64 ? ~0ull >> (64 - TR) : ~0ull);
+    Fill<T, DH, TR>::issue(to, q, a.sq.t, a.D, all, has);
+    Fill<T, DH, TR>::issue(to + kTile, go, a.sgo.t, a.D, all, has);
   };
   int st = split;
   if (st < steps && !needed(st)) st = after(st);
@@ -737,6 +767,7 @@ __global__ __launch_bounds__(256, (waves_of<T, DH>())) void k_attn_dkv(AttnArgs 
         dp = Elem<T>::mma(Tl::row(row, TR + 32 * u, i), vf.get(i), dp);
       }
       f32x16 p;
+      const bool edge = a.causal && here + a.off + rr < k0 + 32 * WN - 1;   // some of these rows do not see some of the workgroup's keys
 #pragma unroll
       for (int q = 0; q < 4; ++q) {
         const int rq = rr + 8 * q + 4 * hi;
@@ -745,7 +776,7 @@ __global__ __launch_bounds__(256, (waves_of<T, DH>())) void k_attn_dkv(AttnArgs 
         for (int i = 0; i < 4; ++i) {
           const int e = 4 * q + i;
           float x = exp2_(__builtin_fmaf(s[e], a.c, PShift<T>::log2 - L[i]));
-          if (a.causal) x = key <= here + a.off + rq + i ? x : 0.f;
+          if (edge) x = key <= here + a.off + rq + i ? x : 0.f;
           p[e] = x;
           s[e] = x * PShift<T>::back * (dp[e] - dl[i]);
         }

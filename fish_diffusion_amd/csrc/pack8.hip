@@ -261,8 +261,8 @@ __global__ __launch_bounds__(256, 2) void k_linear8_wgrad(WgradArgs a) {
       if (a.vec_dy) {
 #pragma unroll
         for (int h = 0; h < NO; ++h)
-          Fill<bf16_t, 128, KT>::issue(to + h * kY, [&](int row) { return n0 + row < ne ? static_cast<const bf16_t*>(a.dy) + (n0 + row) * a.O + o0 + 128 * h : nullptr; },
-                                       a.O - o0 - 128 * h);
+          Fill<bf16_t, 128, KT>::issue(to + h * kY, static_cast<const bf16_t*>(a.dy) + n0 * a.O + o0 + 128 * h, a.O, a.O - o0 - 128 * h,
+                                       n0 + KT <= ne && o0 + 128 * h + 128 <= a.O, [&](int row) { return n0 + row < ne; });
       } else {
 #pragma unroll
         for (int h = 0; h < YR; ++h) {

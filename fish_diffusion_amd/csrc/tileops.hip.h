@@ -105,16 +105,38 @@ static __device__ __attribute__((aligned(16))) unsigned g_zero[4];   // where ro
 // LDS read.  A load has no register output, so nothing can overwrite what is in flight.
 template <typename T, int DH, int TK> struct Fill {
   typedef Tile<T, DH> Tl;
-  static constexpr int N = TK * Tl::CPR / 256, RPI = 64 / Tl::CPR > 0 ? 64 / Tl::CPR : 1;   // wave-instructions per wave, rows each covers
+  static constexpr int N = TK * Tl::CPR / 256, RPI = 64 / Tl::CPR;   // wave-instructions per wave, rows each covers
   static_assert(N * 256 == TK * Tl::CPR && 64 % Tl::CPR == 0, "whole rows per instruction");
-  template <typename F> static __device__ inline void issue(uint4* lds, F&& src, int D) {   // src(row): its address, or null (zeros)
+  // rows t0 ... t0 + TK - 1 of `pitch` elements apart; `all`: every one of them exists and a row is DH elements (uniform), else has(row) says so, and chunks
+  // from D on are zeros
+  template <typename F> static __device__ inline void issue(uint4* lds, const T* t0, long pitch, int D, bool all, F&& has) {
     const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), lane = threadIdx.x & 63;
     const unsigned base = (unsigned)(size_t)(__attribute__((address_space(3))) uint4*)lds;
+    if (all && pitch * TK * (long)sizeof(T) < (1L << 31)) {
+      // one 32-bit lane offset (two where the swizzle alternates from instruction to instruction) on a scalar address: no vector arithmetic per step
+      constexpr int V = 4 * RPI % 16 ? 2 : 1;
+      const unsigned step = 4 * RPI * (unsigned)pitch * (unsigned)sizeof(T);
+      unsigned off[V];
+#pragma unroll
+      for (int v = 0; v < V; ++v) {
+        const int row = wave * RPI + lane / Tl::CPR, c = (lane % Tl::CPR) ^ Tl::swz(row + v * 4 * RPI);
+        off[v] = (unsigned)row * (unsigned)pitch * (unsigned)sizeof(T) + (unsigned)c * 16u;
+      }
+      const char* from = reinterpret_cast<const char*>(t0);
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+        const unsigned to = base + (unsigned)(i * 4 + wave) * 1024u;
+        unsigned keep;
+        asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %3\n\ts_mov_b32 m0, %0"
+                     : "=&s"(keep) : "v"(off[i % V]), "s"(to), "s"(from) : "memory");
+        from += step;
+      }
+      return;
+    }
 #pragma unroll
     for (int i = 0; i < N; ++i) {
       const int row = (i * 4 + wave) * RPI + lane / Tl::CPR, c = (lane % Tl::CPR) ^ Tl::swz(row);
-      const T* p = src(row);
-      const void* from = p && c * Elem<T>::VEC < D ? static_cast<const void*>(p + c * Elem<T>::VEC) : g_zero;
+      const void* from = has(row) && c * Elem<T>::VEC < D ? static_cast<const void*>(t0 + row * pitch + c * Elem<T>::VEC) : g_zero;
       const unsigned to = base + (unsigned)(i * 4 + wave) * 1024u;
       unsigned keep;
       asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off\n\ts_mov_b32 m0, %0"
