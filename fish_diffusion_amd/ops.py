@@ -15,6 +15,7 @@ nothing is kept from one call for the next.  Every call gives the same bits for 
 from __future__ import annotations
 
 import ctypes as C
+import functools
 import math
 from typing import NamedTuple, Optional
 
@@ -110,50 +111,67 @@ def _arg(t: torch.Tensor, vec: int):
     return t, _lib.Bht(at or None, sb, sh, sn)
 
 
-def _workspace(fn, desc, device):
+def _workspace_bytes(fn, *args) -> int:
     n = C.c_size_t()
-    _lib.check(fn(C.byref(desc), C.byref(n)))
-    if not n.value:
-        return None, None, 0
-    ws = torch.empty(n.value, dtype=torch.uint8, device=device)
-    return ws, ws.data_ptr(), n.value
+    _lib.check(fn(*args, C.byref(n)))
+    return n.value
+
+
+def _workspace(n: int, device):
+    return torch.empty(n, dtype=torch.uint8, device=device) if n else None
 
 
 # ------------------------------------------------------------------------------------------------------------- attention
-def _attn_desc(q, k, v, key_mask, causal, scale, what):
-    for t in (q, k, v):
-        if not isinstance(t, torch.Tensor) or t.dim() != 4:
-            raise ValueError(f"{what}: q, k and v must be [batch, heads, length, channels] tensors")
-    dt = _dtype(q, what)
-    B, H, Tq, D = q.shape
-    Hkv, Tk = k.shape[1], k.shape[2]
-    if k.shape != v.shape or k.shape[0] != B or k.shape[3] != D:
-        raise ValueError(f"{what}: q {tuple(q.shape)}, k {tuple(k.shape)} and v {tuple(v.shape)} do not fit together")
+@functools.lru_cache(maxsize=1024)
+def _attn_plan(dtype, qs, ks, vs, causal, scale):
+    """What a call of these types and sizes needs (sizes only, no tensors): its C description, elements per 16 bytes, bytes of workspace each way."""
+    if len(qs) != 4 or len(ks) != 4 or len(vs) != 4:
+        raise ValueError("attention: q, k and v must be [batch, heads, length, channels] tensors")
+    dt = _lib.DTYPES.get(dtype)
+    if dt is None:
+        raise TypeError(f"attention: {dtype} is not one of float32, bfloat16, float16")
+    (B, H, Tq, D), (Hkv, Tk) = qs, ks[1:3]
+    if ks != vs or ks[0] != B or ks[3] != D:
+        raise ValueError(f"attention: q {tuple(qs)}, k {tuple(ks)} and v {tuple(vs)} do not fit together")
     if H == 0 or Hkv == 0 or H % Hkv:
-        raise ValueError(f"{what}: {H} query heads cannot share {Hkv} key / value heads")
+        raise ValueError(f"attention: {H} query heads cannot share {Hkv} key / value heads")
     if D % 8 or not 8 <= D <= 128:
-        raise ValueError(f"{what}: head size {D} is not a multiple of 8 up to 128")
-    scale = 1.0 / math.sqrt(D) if scale is None else float(scale)
+        raise ValueError(f"attention: head size {D} is not a multiple of 8 up to 128")
+    scale = 1.0 / math.sqrt(D) if scale is None else scale
     if not (scale > 0.0 and math.isfinite(scale)):
-        raise ValueError(f"{what}: scale must be positive and finite, got {scale}")
+        raise ValueError(f"attention: scale must be positive and finite, got {scale}")
+    desc = _lib.AttnDesc(dt, B, H, Hkv, Tq, Tk, D, int(causal), scale)
+    lib = _lib.lib()
+    return desc, 4 if dt == 0 else 8, _workspace_bytes(lib.fdx_attn_forward_workspace, desc), _workspace_bytes(lib.fdx_attn_backward_workspace, desc)
+
+
+def _attn_check(q, k, v, key_mask, causal, scale):
+    for t in (q, k, v):
+        if not isinstance(t, torch.Tensor):
+            raise ValueError("attention: q, k and v must be [batch, heads, length, channels] tensors")
+    plan = _attn_plan(q.dtype, q.shape, k.shape, v.shape, bool(causal), None if scale is None else float(scale))
+    dev = q.get_device()
     if key_mask is not None:
         if key_mask.dtype not in (torch.bool, torch.uint8):
-            raise TypeError(f"{what}: key_mask must be bool or uint8 (true = masked), got {key_mask.dtype}")
-        if key_mask.shape != (B, Tk):
-            raise ValueError(f"{what}: key_mask {tuple(key_mask.shape)} is not [batch, keys] = {(B, Tk)}")
-        if key_mask.device != q.device:
-            raise ValueError(f"{what}: key_mask is on {key_mask.device}, expected {q.device}")
+            raise TypeError(f"attention: key_mask must be bool or uint8 (true = masked), got {key_mask.dtype}")
+        if key_mask.shape != (q.shape[0], k.shape[2]):
+            raise ValueError(f"attention: key_mask {tuple(key_mask.shape)} is not [batch, keys] = {(q.shape[0], k.shape[2])}")
+        if key_mask.get_device() != dev:
+            raise ValueError(f"attention: key_mask is on {key_mask.device}, expected {q.device}")
         key_mask = key_mask.contiguous()
-    if not q.is_cuda:
-        _lib.require_gpu(q, f"{what} q")
-    _same(q, what, k=k, v=v)
-    return _lib.AttnDesc(dt, B, H, Hkv, Tq, Tk, D, int(bool(causal)), scale), key_mask, (4 if dt == 0 else 8)
+    if dev < 0:
+        _lib.require_gpu(q, "attention q")
+    if k.get_device() != dev or v.get_device() != dev or k.dtype is not q.dtype or v.dtype is not q.dtype:
+        _same(q, "attention", k=k, v=v)
+    return plan, key_mask
 
 
-def _like_rows(t: torch.Tensor) -> torch.Tensor:
-    """An uninitialised tensor of t's [B, H, T, D] shape that lies in memory as [B, T, H, D]: joining the heads afterwards is a view."""
+def _new_rows(t: torch.Tensor):
+    """An uninitialised tensor of t's [B, H, T, D] shape that lies in memory as [B, T, H, D] -- joining the heads afterwards is a view -- and its description."""
     B, H, T, D = t.shape
-    return torch.empty(B, T, H, D, dtype=t.dtype, device=t.device).transpose(1, 2)
+    strides = (T * H * D, D, H * D, 1)
+    new = torch.empty_strided(t.shape, strides, dtype=t.dtype, device=t.device)
+    return new, _lib.Bht(new.data_ptr() or None, *strides[:3])
 
 
 def attention_forward(q, k, v, key_mask=None, causal=False, scale=None):
@@ -163,15 +181,14 @@ def attention_forward(q, k, v, key_mask=None, causal=False, scale=None):
     key_mask [B, Tk], true = masked (whatever masked keys and values hold, NaN included, is never used); causal: query i sees keys up to
     i + Tk - Tq; scale defaults to D ** -0.5.  A row that sees no key is 0 (lse -inf).  Any strides; channels that are not contiguous or not
     16-byte aligned are copied first.  No autograd graph (`attention` builds one)."""
-    desc, key_mask, vec = _attn_desc(q, k, v, key_mask, causal, scale, "attention")
+    (desc, vec, n, _), key_mask = _attn_check(q, k, v, key_mask, causal, scale)
     (q, aq), (k, ak), (v, av) = _arg(q, vec), _arg(k, vec), _arg(v, vec)
     device = q.device
-    out = _like_rows(q)
+    out, ao = _new_rows(q)
     lse = torch.empty(q.shape[:3], dtype=torch.float32, device=device)
-    h, lib = _handle(device), _lib.lib()
-    ws, wp, n = _workspace(lib.fdx_attn_forward_workspace, desc, device)
+    h, ws = _handle(device), _workspace(n, device)
     with h.lock:
-        rc = lib.fdx_attn_forward(h.h, desc, aq, ak, av, None if key_mask is None else key_mask.data_ptr(), _arg(out, vec)[1], lse.data_ptr(), wp, n, _stream(h))
+        rc = _lib.lib().fdx_attn_forward(h.h, desc, aq, ak, av, _p(key_mask), ao, lse.data_ptr(), _p(ws), n, _stream(h))
         if rc:
             _lib.check(rc, h.h)
     return out, lse
@@ -180,20 +197,19 @@ def attention_forward(q, k, v, key_mask=None, causal=False, scale=None):
 def attention_backward(grad_out, q, k, v, out, lse, key_mask=None, causal=False, scale=None):
     """(dq, dk, dv) of `attention_forward` called with the same arguments, from grad_out and its results.  dk / dv are summed over the query
     heads that share a key / value head; masked keys get 0, rows that see no key give 0 whatever grad_out holds there."""
-    desc, key_mask, vec = _attn_desc(q, k, v, key_mask, causal, scale, "attention_backward")
+    (desc, vec, _, n), key_mask = _attn_check(q, k, v, key_mask, causal, scale)
     _same(q, "attention_backward", grad_out=grad_out, out=out)
     if grad_out.shape != q.shape or out.shape != q.shape:
         raise ValueError(f"attention_backward: grad_out {tuple(grad_out.shape)} and out {tuple(out.shape)} must have q's shape {tuple(q.shape)}")
-    if lse.shape != q.shape[:3] or lse.dtype != torch.float32 or lse.device != q.device:
-        raise ValueError(f"attention_backward: lse must be the forward's float32 {tuple(q.shape[:3])} on {q.device}")
+    device = q.device
+    if lse.shape != q.shape[:3] or lse.dtype != torch.float32 or lse.device != device:
+        raise ValueError(f"attention_backward: lse must be the forward's float32 {tuple(q.shape[:3])} on {device}")
     (grad_out, ag), (q, aq), (k, ak), (v, av), (out, ao) = (_arg(t, vec) for t in (grad_out, q, k, v, out))
     lse = lse.contiguous()
-    dq, dk, dv = _like_rows(q), _like_rows(k), _like_rows(v)
-    h, lib = _handle(q.device), _lib.lib()
-    ws, wp, n = _workspace(lib.fdx_attn_backward_workspace, desc, q.device)
+    (dq, adq), (dk, adk), (dv, adv) = _new_rows(q), _new_rows(k), _new_rows(v)
+    h, ws = _handle(device), _workspace(n, device)
     with h.lock:
-        rc = lib.fdx_attn_backward(h.h, desc, ag, aq, ak, av, ao, lse.data_ptr(), None if key_mask is None else key_mask.data_ptr(),
-                                   _arg(dq, vec)[1], _arg(dk, vec)[1], _arg(dv, vec)[1], wp, n, _stream(h))
+        rc = _lib.lib().fdx_attn_backward(h.h, desc, ag, aq, ak, av, ao, lse.data_ptr(), _p(key_mask), adq, adk, adv, _p(ws), n, _stream(h))
         if rc:
             _lib.check(rc, h.h)
     return dq, dk, dv
@@ -232,6 +248,7 @@ class ResidualNormGrads(NamedTuple):
 
 
 _KINDS = {"layer": 0, "rms": 1}
+_NO_NORM = (None, None)
 
 
 def _packed_rows(t: Optional[torch.Tensor]) -> Optional[torch.Tensor]:
@@ -241,53 +258,61 @@ def _packed_rows(t: Optional[torch.Tensor]) -> Optional[torch.Tensor]:
     return t if t.is_contiguous() and not t.data_ptr() & 15 else _copy(t)
 
 
-def _norm_args(x, block, gate, residual_scale, post_norm, pre_norm, kind, eps, what):
-    if not torch.is_tensor(x) or not torch.is_tensor(block) or x.dim() < 1 or x.shape != block.shape:
-        raise ValueError(f"{what}: x and block must be tensors of one shape [..., channels]")
-    dt = _dtype(x, what)
-    C_ = x.shape[-1]
-    if not 1 <= C_ <= 8192:
-        raise ValueError(f"{what}: {C_} channels are not within 1 ... 8192")
+@functools.lru_cache(maxsize=1024)
+def _norm_plan(dtype, shape, param_dtypes, param_shapes, gate_dtype, gate_shape, residual_scale, kind, eps):
+    """The C description of a call of these types and sizes, and its backward pass's bytes of workspace."""
+    dt = _lib.DTYPES.get(dtype)
+    if dt is None:
+        raise TypeError(f"residual_norm: {dtype} is not one of float32, bfloat16, float16")
+    if len(shape) < 1 or not 1 <= shape[-1] <= 8192:
+        raise ValueError(f"residual_norm: {tuple(shape)} does not end in 1 ... 8192 channels")
+    C_, N = shape[-1], math.prod(shape[:-1])
     if kind not in _KINDS:
-        raise ValueError(f"{what}: kind must be 'layer' or 'rms', got {kind!r}")
+        raise ValueError(f"residual_norm: kind must be 'layer' or 'rms', got {kind!r}")
     if not (math.isfinite(residual_scale) and eps >= 0.0 and math.isfinite(eps)):
-        raise ValueError(f"{what}: residual_scale must be finite and eps finite and not negative")
-    params = []
-    for name, wb in (("post_norm", post_norm), ("pre_norm", pre_norm)):
-        w, b = (None, None) if wb is None else wb
-        if wb is not None and w is None:
-            raise ValueError(f"{what}: {name} must be (weight, bias or None)")
-        params += [w, b]
-    pdt = {p.dtype for p in params if p is not None} or {x.dtype}
-    if len(pdt) > 1 or not pdt <= {x.dtype, torch.float32}:
-        raise ValueError(f"{what}: the norms' weights and biases must all be {x.dtype} or all float32, got {sorted(map(str, pdt))}")
-    for p in params:
-        if p is not None and p.shape != (C_,):
-            raise ValueError(f"{what}: a norm's weight / bias has shape {tuple(p.shape)}, expected {(C_,)}")
-    N = x.numel() // C_
+        raise ValueError("residual_norm: residual_scale must be finite and eps finite and not negative")
+    pdt = set(t for t in param_dtypes if t is not None) or {dtype}
+    if len(pdt) > 1 or not pdt <= {dtype, torch.float32}:
+        raise ValueError(f"residual_norm: the norms' weights and biases must all be {dtype} or all float32, got {sorted(map(str, pdt))}")
+    for sh in param_shapes:
+        if sh is not None and sh != (C_,):
+            raise ValueError(f"residual_norm: a norm's weight / bias has shape {tuple(sh)}, expected {(C_,)}")
     rows = 0
-    if gate is not None:
-        if gate.dtype not in (x.dtype, torch.float32):
-            raise ValueError(f"{what}: gate must be {x.dtype} or float32, got {gate.dtype}")
-        if gate.shape == x.shape and x.dim() > 1:
+    if gate_shape is not None:
+        if gate_dtype not in (dtype, torch.float32):
+            raise ValueError(f"residual_norm: gate must be {dtype} or float32, got {gate_dtype}")
+        if gate_shape == shape and len(shape) > 1:
             rows = 1
-        elif gate.shape == (C_,):
+        elif gate_shape == (C_,):
             rows = max(N, 1)
-        elif x.dim() == 3 and tuple(gate.shape) in ((x.shape[0], C_), (x.shape[0], 1, C_)):
-            rows = max(x.shape[1], 1)
+        elif len(shape) == 3 and tuple(gate_shape) in ((shape[0], C_), (shape[0], 1, C_)):
+            rows = max(shape[1], 1)
         else:
-            raise ValueError(f"{what}: gate {tuple(gate.shape)} is none of [channels], [batch, channels], [batch, 1, channels] and x's {tuple(x.shape)}")
-    device = x.device
+            raise ValueError(f"residual_norm: gate {tuple(gate_shape)} is none of [channels], [batch, channels], [batch, 1, channels] and x's {tuple(shape)}")
+    desc = _lib.ResnormDesc(dt, _lib.DTYPES[next(iter(pdt))], dt if gate_shape is None else _lib.DTYPES[gate_dtype], N, C_, rows, _KINDS[kind],
+                            residual_scale, eps)
+    return desc, _workspace_bytes(_lib.lib().fdx_resnorm_backward_workspace, desc)
+
+
+def _norm_args(x, block, gate, residual_scale, post_norm, pre_norm, kind, eps):
+    if not isinstance(x, torch.Tensor) or not isinstance(block, torch.Tensor) or x.shape != block.shape:
+        raise ValueError("residual_norm: x and block must be tensors of one shape [..., channels]")
+    pw, pb = post_norm or _NO_NORM
+    nw, nb = pre_norm or _NO_NORM
+    if (post_norm and pw is None) or (pre_norm and nw is None):
+        raise ValueError("residual_norm: post_norm and pre_norm must be None or (weight, bias or None)")
+    params = (pw, pb, nw, nb)
+    plan = _norm_plan(x.dtype, x.shape, tuple([p if p is None else p.dtype for p in params]), tuple([p if p is None else p.shape for p in params]),
+                      None if gate is None else gate.dtype, None if gate is None else gate.shape, float(residual_scale), kind, float(eps))
+    if block.dtype is not x.dtype:
+        raise ValueError(f"residual_norm: block is {block.dtype}, x {x.dtype}")
+    dev = x.get_device()
     for t in (block, gate, *params):
-        if t is not None and t.device != device:
-            raise ValueError(f"{what}: tensors on {t.device} and {device}")
-    if not x.is_cuda:
-        _lib.require_gpu(x, f"{what} x")
-    if block.dtype != x.dtype:
-        raise ValueError(f"{what}: block is {block.dtype}, x {x.dtype}")
-    desc = _lib.ResnormDesc(dt, _lib.DTYPES[next(iter(pdt))], dt if gate is None else _lib.DTYPES[gate.dtype], N, C_, rows, _KINDS[kind],
-                            float(residual_scale), float(eps))
-    return desc, [_packed_rows(p) for p in params]
+        if t is not None and t.get_device() != dev:
+            raise ValueError(f"residual_norm: tensors on {t.device} and {x.device}")
+    if dev < 0:
+        _lib.require_gpu(x, "residual_norm x")
+    return plan, [p if p is None else _packed_rows(p) for p in params]
 
 
 def residual_norm_forward(x, block, gate=None, residual_scale=1.0, post_norm=None, pre_norm=None, kind="layer", eps=1e-5, need_h=True):
@@ -299,23 +324,25 @@ def residual_norm_forward(x, block, gate=None, residual_scale=1.0, post_norm=Non
     written."""
     if not need_h and pre_norm is None:
         raise ValueError("residual_norm: need_h=False without a pre_norm leaves no result")
-    desc, (pw, pb, nw, nb) = _norm_args(x, block, gate, residual_scale, post_norm, pre_norm, kind, eps, "residual_norm")
+    (desc, _), (pw, pb, nw, nb) = _norm_args(x, block, gate, residual_scale, post_norm, pre_norm, kind, eps)
     x, block, gate = _packed_rows(x), _packed_rows(block), _packed_rows(gate)
     h_out = torch.empty_like(x) if need_h else None
     y = torch.empty_like(x) if nw is not None else None
-    stats = torch.empty((*x.shape[:-1], 4), dtype=torch.float32, device=x.device)
+    stats = torch.empty(x.shape[:-1] + (4,), dtype=torch.float32, device=x.device)
     if x.numel():
-        h, lib = _handle(x.device), _lib.lib()
+        h = _handle(x.device)
         with h.lock:
-            _lib.check(lib.fdx_resnorm_forward(h.h, desc, *(_p(t) for t in (x, block, gate, pw, pb, nw, nb, h_out, y, stats)),
-                                               _stream(h)), h.h)
+            rc = _lib.lib().fdx_resnorm_forward(h.h, desc, x.data_ptr(), block.data_ptr(), _p(gate), _p(pw), _p(pb), _p(nw), _p(nb), _p(h_out), _p(y),
+                                                stats.data_ptr(), _stream(h))
+            if rc:
+                _lib.check(rc, h.h)
     return h_out, y, stats
 
 
 def residual_norm_backward(grad_h, grad_y, x, block, stats, gate=None, residual_scale=1.0, post_norm=None, pre_norm=None, kind="layer", eps=1e-5):
     """`ResidualNormGrads` from the gradients of h and y (either may be None) and the forward's arguments and stats.  Where there is no gate, no post norm and
     residual_scale is 1, dx and dblock are equal and are ONE tensor.  The gate's gradient has the gate's shape."""
-    desc, (pw, pb, nw, nb) = _norm_args(x, block, gate, residual_scale, post_norm, pre_norm, kind, eps, "residual_norm_backward")
+    (desc, n), (pw, pb, nw, nb) = _norm_args(x, block, gate, residual_scale, post_norm, pre_norm, kind, eps)
     for name, g in (("grad_h", grad_h), ("grad_y", grad_y)):
         if g is not None and (g.shape != x.shape or g.dtype != x.dtype or g.device != x.device):
             raise ValueError(f"residual_norm_backward: {name} must be {x.dtype} {tuple(x.shape)} on {x.device}")
@@ -333,11 +360,12 @@ def residual_norm_backward(grad_h, grad_y, x, block, stats, gate=None, residual_
             if t is not None:
                 t.zero_()
     else:
-        h, lib = _handle(x.device), _lib.lib()
-        ws, wp, n = _workspace(lib.fdx_resnorm_backward_workspace, desc, x.device)
+        h, ws = _handle(x.device), _workspace(n, x.device)
         with h.lock:
-            _lib.check(lib.fdx_resnorm_backward(h.h, desc, *(_p(t) for t in (grad_h, grad_y, x, block, gate_c, pw, pb, nw, nb, stats, dx, dblock,
-                                                                                           dgate, *grads)), wp, n, _stream(h)), h.h)
+            rc = _lib.lib().fdx_resnorm_backward(h.h, desc, *[_p(t) for t in (grad_h, grad_y, x, block, gate_c, pw, pb, nw, nb, stats, dx, dblock, dgate, *grads)],
+                                                 _p(ws), n, _stream(h))
+            if rc:
+                _lib.check(rc, h.h)
     return ResidualNormGrads(dx, dblock, dgate, *grads)
 
 
@@ -391,8 +419,7 @@ def _packed_ok(p: Packed8, what: str) -> Packed8:
 
 
 def _new_packed(x: torch.Tensor) -> Packed8:
-    return Packed8(torch.empty(x.shape, dtype=torch.int8, device=x.device),
-                   torch.empty((*x.shape[:-1], (x.shape[-1] + 31) // 32), dtype=torch.uint8, device=x.device))
+    return Packed8(torch.empty_like(x, dtype=torch.int8), torch.empty(x.shape[:-1] + ((x.shape[-1] + 31) // 32,), dtype=torch.uint8, device=x.device))
 
 
 def pack8(x) -> Packed8:
@@ -407,7 +434,9 @@ def pack8(x) -> Packed8:
     p = _new_packed(x)
     h = _handle(x.device)
     with h.lock:
-        _lib.check(_lib.lib().fdx_pack8(h.h, dt, _p(x), N, C_, _p(p.codes), _p(p.exponents), _stream(h)), h.h)
+        rc = _lib.lib().fdx_pack8(h.h, dt, x.data_ptr(), N, C_, p.codes.data_ptr(), p.exponents.data_ptr(), _stream(h))
+        if rc:
+            _lib.check(rc, h.h)
     return p
 
 
@@ -442,12 +471,12 @@ def linear8_weight_grad(dy, packed: Packed8, bias=True, dtype=None):
     dy = _packed_rows(dy)
     dw = torch.empty(O, I, dtype=dtype, device=dy.device)
     db = torch.empty(O, dtype=dtype, device=dy.device) if bias else None
-    h, lib, n = _handle(dy.device), _lib.lib(), C.c_size_t()
-    _lib.check(lib.fdx_linear8_weight_grad_workspace(dt, N, O, I, C.byref(n)))
-    ws = torch.empty(n.value, dtype=torch.uint8, device=dy.device)
+    h, lib = _handle(dy.device), _lib.lib()
+    n = _workspace_bytes(lib.fdx_linear8_weight_grad_workspace, dt, N, O, I)
+    ws = _workspace(n, dy.device)
     with h.lock:
         _lib.check(lib.fdx_linear8_weight_grad(h.h, dt, _p(dy), _p(p.codes), _p(p.exponents), N, O, I, _lib.DTYPES[dtype], _p(dw),
-                                               _p(db), _p(ws), n.value, _stream(h)), h.h)
+                                               _p(db), _p(ws), n, _stream(h)), h.h)
     return dw, db
 
 
