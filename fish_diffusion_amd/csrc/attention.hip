@@ -345,32 +345,43 @@ __global__ __launch_bounds__(256, (waves_of<T, DH>())) void k_attn_fwd(AttnArgs 
   }
 }
 
-// splits of the keys joined: one wave per row, two channels a lane, in split order
+// splits of the keys joined: one wave per row, two channels a lane.  Every lane takes one split's (reference, sum) -- at most 64 -- and the weights travel by
+// lane reads, so the rows of O are the only chain: eight loads in flight.
 template <typename T> __global__ __launch_bounds__(256) void k_attn_join(AttnArgs a) {
   const int lane = threadIdx.x & 63;
   const long row = (long)blockIdx.x * 4 + (threadIdx.x >> 6);
   if (row >= (long)a.B * a.Hkv * a.R) return;
   const long bh = row / a.R, r = row - bh * a.R;
   const float2* ml = reinterpret_cast<const float2*>(a.part + (long)a.B * a.Hkv * a.splits * a.R * a.D) + bh * a.splits * a.R + r;
-  float M = -inf(), L = 0.f, o0 = 0.f, o1 = 0.f;
-  for (int s = 0; s < a.splits; ++s) M = fmaxf(M, ml[(long)s * a.R].x);
-  const float Mz = M == -inf() ? 0.f : M;
-  for (int s = 0; s < a.splits; ++s) {
-    const float2 v = ml[(long)s * a.R];
-    const float w = exp2_(v.x - Mz);
-    L += v.y * w;
-    if (2 * lane < a.D) {
-      const float2 o = *reinterpret_cast<const float2*>(a.part + ((bh * a.splits + s) * a.R + r) * a.D + 2 * lane);
-      o0 += o.x * w;
-      o1 += o.y * w;
+  const float2 mine = lane < a.splits ? ml[(long)lane * a.R] : float2{-inf(), 0.f};
+  const float* const p = a.part + (bh * a.splits * a.R + r) * a.D + 2 * lane;
+  const long pitch = (long)a.R * a.D;
+  const bool in = 2 * lane < a.D;
+  float M = mine.x;
+#pragma unroll
+  for (int d = 1; d < 64; d *= 2) M = fmaxf(M, __shfl_xor(M, d, 64));
+  const float w = exp2_(mine.x - (M == -inf() ? 0.f : M));
+  float L = mine.y * w;
+#pragma unroll
+  for (int d = 1; d < 64; d *= 2) L += __shfl_xor(L, d, 64);
+  float o0 = 0.f, o1 = 0.f;
+  for (int s = 0; s < a.splits; s += 8) {
+    float2 o[8];
+#pragma unroll
+    for (int q = 0; q < 8; ++q) o[q] = in && s + q < a.splits ? *reinterpret_cast<const float2*>(p + (s + q) * pitch) : float2{0.f, 0.f};
+#pragma unroll
+    for (int q = 0; q < 8; ++q) {
+      const float ws = __shfl(w, (s + q) & 63, 64);
+      o0 = __builtin_fmaf(o[q].x, ws, o0);
+      o1 = __builtin_fmaf(o[q].y, ws, o1);
     }
   }
   const float f = L == 0.f ? 0.f : 1.f / L;
   const int b = (int)(bh / a.Hkv), hk = (int)(bh % a.Hkv), g = (int)r / a.Tq, t = (int)r - g * a.Tq;
-  if (2 * lane < a.D) {
-    T* p = static_cast<T*>(a.o) + b * a.so.b + (hk * a.G + g) * a.so.h + t * a.so.t + 2 * lane;
-    p[0] = (T)(o0 * f);
-    p[1] = (T)(o1 * f);
+  if (in) {
+    T* out = static_cast<T*>(a.o) + b * a.so.b + (hk * a.G + g) * a.so.h + t * a.so.t + 2 * lane;
+    out[0] = (T)(o0 * f);
+    out[1] = (T)(o1 * f);
   }
   if (lane == 0) a.lse[row] = L == 0.f ? -inf() : (M + __builtin_amdgcn_logf(L) - PShift<T>::log2) * kLn2;
 }
@@ -633,17 +644,27 @@ template <typename T> __global__ __launch_bounds__(256) void k_attn_join_dq(Attn
   if (kMend && lane == 0) a.delta[row] += left;
 }
 
-// partial sums [B * Hkv][splits][n rows][D] of one gradient joined in split order; rows are (g, t) with G = rows / T heads per kv head
-struct JoinArgs { const float* part; void* out; Str so; int Hkv, rows, T, D, splits; long nvec; };
-template <typename T> __global__ __launch_bounds__(256) void k_attn_join_sum(JoinArgs a) {
-  const long i = (long)blockIdx.x * 256 + threadIdx.x;
-  if (i >= a.nvec) return;
-  const int d4 = a.D / 4, d = (int)(i % d4) * 4;
-  const long row = i / d4, bh = row / a.rows;
-  const int r = (int)(row - bh * a.rows), G = a.rows / a.T, g = r / a.T, t = r - g * a.T;
+// partial sums [B * Hkv][splits][Tk][D] of dk and, behind them, dv joined in split order: four channels a thread, eight loads in flight
+template <typename T> __global__ __launch_bounds__(256) void k_attn_join_dkv(AttnArgs a) {
+  const int d4 = a.D / 4;
+  const long n = (long)a.B * a.Hkv * a.Tk * d4;
+  long i = (long)blockIdx.x * 256 + threadIdx.x;
+  const bool second = i >= n;
+  if (second) i -= n;
+  if (i >= n) return;
+  const int d = (int)(i % d4) * 4;
+  const long row = i / d4, bh = row / a.Tk, key = row - bh * a.Tk, pitch = (long)a.Tk * a.D;
+  const float* const p = a.part + (second ? n * 4 * a.splits : 0) + (bh * a.splits * a.Tk + key) * a.D + d;
   f32x4 v = {0, 0, 0, 0};
-  for (int s = 0; s < a.splits; ++s) v += *reinterpret_cast<const f32x4*>(a.part + ((bh * a.splits + s) * a.rows + r) * a.D + d);
-  store4<T>(static_cast<T*>(a.out) + (bh / a.Hkv) * a.so.b + ((bh % a.Hkv) * G + g) * a.so.h + t * a.so.t + d, v[0], v[1], v[2], v[3]);
+  for (int s = 0; s < a.splits; s += 8) {
+    f32x4 t[8];
+#pragma unroll
+    for (int q = 0; q < 8; ++q) t[q] = s + q < a.splits ? *reinterpret_cast<const f32x4*>(p + (s + q) * pitch) : f32x4{0, 0, 0, 0};
+#pragma unroll
+    for (int q = 0; q < 8; ++q) v += t[q];
+  }
+  const Str& st = second ? a.sdv : a.sdk;
+  store4<T>(static_cast<T*>(second ? a.dv : a.dk) + (bh / a.Hkv) * st.b + (bh % a.Hkv) * st.h + key * st.t + d, v[0], v[1], v[2], v[3]);
 }
 
 // dk, dv: WN waves own 32 keys each, the other factor (WR) shares those keys and takes RT rows each of every step
@@ -916,10 +937,6 @@ template <typename T, int DH> struct RunFwd {
 };
 
 template <typename T, int DH> struct RunBwd {
-  static hipError_t join(const AttnArgs& a, const float* part, void* out, const Str& so, int rows, int T_, hipStream_t s) {
-    JoinArgs j{part, out, so, a.Hkv, rows, T_, a.D, a.splits, (long)a.B * a.Hkv * rows * (a.D / 4)};
-    return launch(k_attn_join_sum<T>, (unsigned)((j.nvec + 255) / 256), 256, j, s);
-  }
   static hipError_t go(AttnArgs& a, const Plan& pq, const Plan& pk, float* part, hipStream_t s) {
     hipError_t e = hipSuccess;
     a.part = part;
@@ -933,11 +950,8 @@ template <typename T, int DH> struct RunBwd {
       a.tiles = pk.tiles; a.splits = pk.splits;
       const unsigned grid = (unsigned)((long)a.B * a.Hkv * pk.tiles * pk.splits);
       e = pk.narrow ? launch(k_attn_dkv<T, DH, 1, 32>, grid, 256, a, s) : launch(k_attn_dkv<T, DH, 4, (DH * sizeof(T) >= 256 ? 32 : 64)>, grid, 256, a, s);
-      if (e == hipSuccess && pk.splits > 1) {
-        const size_t half = (size_t)a.B * a.Hkv * a.splits * a.Tk * a.D;
-        e = join(a, part, a.dk, a.sdk, a.Tk, a.Tk, s);
-        if (e == hipSuccess) e = join(a, part + half, a.dv, a.sdv, a.Tk, a.Tk, s);
-      }
+      if (e == hipSuccess && pk.splits > 1)
+        e = launch(k_attn_join_dkv<T>, (unsigned)(((long)a.B * a.Hkv * a.Tk * (a.D / 4) * 2 + 255) / 256), 256, a, s);
     }
     return e;
   }
