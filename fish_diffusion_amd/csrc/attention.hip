@@ -290,6 +290,7 @@ __global__ __launch_bounds__(256, (waves_of<T, DH>())) void k_attn_fwd(AttnArgs 
         sum += s[u][e];
       }
     l += sum;
+    __builtin_amdgcn_s_setprio(1);   // this wave's products before the other one's exponentials, which then run under them: 214 -> 209 us
 #pragma unroll
     for (int u = 0; u < NU; ++u)
 #pragma unroll
@@ -298,6 +299,7 @@ __global__ __launch_bounds__(256, (waves_of<T, DH>())) void k_attn_fwd(AttnArgs 
 #pragma unroll
         for (int m = 0; m < MT; ++m) acc[m] = Elem<T>::mma(Tl::col(col, V0 + 32 * u + KS * p, m), pf, acc[m]);
       }
+    __builtin_amdgcn_s_setprio(0);
   }
   l = half_sum(l);
 
@@ -508,11 +510,13 @@ __global__ __launch_bounds__(256, (waves_of<T, DH>())) void k_attn_dq(AttnArgs a
 #pragma unroll
     for (int u = 0; u < NU; ++u) {
       f32x16 s = {0}, dp = {0};
+      __builtin_amdgcn_s_setprio(1);   // as in the forward, around the products with the longer chains: 377 -> 348 us
 #pragma unroll
       for (int i = 0; i < NS; ++i) {
         s = Elem<T>::mma(Tl::row(row, 32 * u, i), qf[i], s);
         dp = Elem<T>::mma(Tl::row(row, V0 + 32 * u, i), gf.get(i), dp);
       }
+      __builtin_amdgcn_s_setprio(0);
 #pragma unroll
       for (int e = 0; e < 16; ++e) s[e] = exp2_(__builtin_fmaf(s[e], a.c, PShift<T>::log2 - L));
       if (!whole) {
@@ -803,6 +807,7 @@ __global__ __launch_bounds__(256, (waves_of<T, DH>())) void k_attn_dkv(AttnArgs 
         }
       }
       if constexpr (kScaled) rs.fit<MT>(s, dk);
+      __builtin_amdgcn_s_setprio(1);   // as in the forward: 373 -> 367 us
 #pragma unroll
       for (int i = 0; i < NP; ++i) {
         const frag pf = acc_frag<T>(p, i), df = acc_frag<T>(s, i);
@@ -812,6 +817,7 @@ __global__ __launch_bounds__(256, (waves_of<T, DH>())) void k_attn_dkv(AttnArgs 
           dk[m] = Elem<T>::mma(Tl::col(col, 32 * u + KS * i, m), df, dk[m]);
         }
       }
+      __builtin_amdgcn_s_setprio(0);
     }
   }
   float f = a.scale, fv = PShift<T>::back;
