@@ -54,14 +54,16 @@ __device__ inline float half_sum(float x) {
 }
 
 // workgroup -> (batch and kv head, tile, split).  Workgroups go to the 8 XCDs in turn: where the heads divide, all tiles of a head run on one
-// XCD and find its K / V in that XCD's L2.  Late (causal: long) tiles start first.
-__device__ inline void decode(const AttnArgs& a, int& bh, int& tile, int& split) {
+// XCD and find its K / V in that XCD's L2.  Causal tiles start in the order of their length, the G heads' longest first: the grid then has G times
+// ceil(tiles / G) places and those past the last tile end at once (2 x 16 / 4 heads x 4096 x 128: forward 212 -> MEASURED us against head after head).
+__device__ inline void decode(const AttnArgs& a, int G, int& bh, int& tile, int& split) {
   const int nb = a.B * a.Hkv, per = a.tiles * a.splits, i = blockIdx.x;
   int j;
   if (nb % 8 == 0) { bh = (i & 7) + 8 * ((i >> 3) / per); j = (i >> 3) % per; }
   else { bh = i / per; j = i % per; }
   split = j % a.splits;
-  tile = a.tiles - 1 - j / a.splits;
+  j /= a.splits;
+  tile = a.causal ? j % G * (a.tiles / G) + a.tiles / G - 1 - j / G : j;
 }
 
 // one past the last key any row of [r0, r1] sees
@@ -190,7 +192,8 @@ __global__ __launch_bounds__(256, (waves_of<T, DH>())) void k_attn_fwd(AttnArgs 
   __shared__ __attribute__((aligned(1024))) uint4 smem[2 * S * kTile > kMerge ? 2 * S * kTile : kMerge];       // S stages of K and V
   __shared__ float ml[2][4][32];
   int bh, tile, split;
-  decode(a, bh, tile, split);
+  decode(a, a.G, bh, tile, split);
+  if (tile * 32 * WQ >= a.R) return;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wq = wave / WK, wk = wave % WK, hi = lane >> 5;
   const int b = bh / a.Hkv, hk = bh % a.Hkv;
   const int r0 = tile * 32 * WQ, r = r0 + wq * 32 + (lane & 31), rc = min(r, a.R - 1), g = rc / a.Tq, t = rc - g * a.Tq;
@@ -425,7 +428,8 @@ __global__ __launch_bounds__(256, (waves_of<T, DH>())) void k_attn_dq(AttnArgs a
   constexpr bool PARK = parked<T, DH>();
   __shared__ uint4 own[PARK ? WQ * NS * 64 : 1];
   int bh, tile, split;
-  decode(a, bh, tile, split);
+  decode(a, a.G, bh, tile, split);
+  if (tile * 32 * WQ >= a.R) return;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wq = wave / WK, wk = wave % WK, hi = lane >> 5;
   const int b = bh / a.Hkv, hk = bh % a.Hkv;
   const int r0 = tile * 32 * WQ, r = r0 + wq * 32 + (lane & 31), rc = min(r, a.R - 1), g = rc / a.Tq, t = rc - g * a.Tq;
@@ -686,8 +690,8 @@ __global__ __launch_bounds__(256, (waves_of<T, DH>())) void k_attn_dkv(AttnArgs 
   constexpr bool PARK = parked<T, DH>();
   __shared__ uint4 own[PARK ? WN * NS * 64 : 1];
   int bh, tile, split;
-  decode(a, bh, tile, split);
-  tile = a.tiles - 1 - tile;   // early keys are the long ones here
+  decode(a, 1, bh, tile, split);
+  if (a.causal) tile = a.tiles - 1 - tile;   // early keys are the long ones here
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wn = wave / WR, wr = wave % WR, hi = lane >> 5;
   const int b = bh / a.Hkv, hk = bh % a.Hkv;
   const int k0 = tile * 32 * WN, key = k0 + wn * 32 + (lane & 31);
@@ -864,13 +868,14 @@ namespace {
 // whose waves share the keys; and while even those leave CUs empty the other axis is split over workgroups and joined.  512 workgroups are resident;
 // causal tiles differ in length by up to all of it, and twice as many workgroups as are resident, long ones first, even that out.
 struct Plan { int narrow, tiles, splits; };   // narrow: 32 rows per workgroup
-Plan plan_of(int nb, int rows, int across, bool causal) {
+Plan plan_of(int nb, int rows, int across, bool causal, int G) {   // G: heads in the rows
   Plan p;
   const long n32 = (long)nb * ((rows + 31) / 32);
   p.narrow = n32 <= 512;
   p.tiles = p.narrow ? (rows + 31) / 32 : (rows + 127) / 128;
   const long base = std::max<long>(1, (long)nb * p.tiles), want = causal ? 1024 : 512;
   const int steps = p.narrow ? (across + 127) / 128 : (across + 63) / 64;
+  if (causal) p.tiles = (p.tiles + G - 1) / G * G;
   long s = base > want * 3 / 4 ? 1 : (want + base / 2) / base;
   s = std::min<long>(s, steps / 2);
   p.splits = (int)std::max<long>(1, std::min<long>(s, 64));
@@ -886,7 +891,7 @@ const char* check(const fdx_attn_desc* d) {
   if (!(d->scale > 0.f) || !std::isfinite(d->scale)) return "scale must be positive and finite";
   const long R = (long)(d->heads / d->kv_heads) * d->q_len, nb = (long)d->batch * d->kv_heads;
   if (R > INT_MAX / 2 || d->k_len > INT_MAX / 2) return "too many rows for one key / value head";
-  if (nb * ((R + 31) / 32) > INT_MAX / 64 || nb * (((long)d->k_len + 31) / 32) > INT_MAX / 64) return "too many tiles for one launch";
+  if (nb * ((R + 31) / 32 + d->heads) > INT_MAX / 64 || nb * (((long)d->k_len + 31) / 32) > INT_MAX / 64) return "too many tiles for one launch";
   return nullptr;
 }
 
@@ -969,7 +974,7 @@ extern "C" int fdx_attn_forward_workspace(const fdx_attn_desc* d, size_t* bytes)
   if (const char* why = check(d)) return fail(nullptr, FDX_E_ARG, "fdx_attn_forward_workspace: %s", why);
   if (!bytes) return fail(nullptr, FDX_E_ARG, "fdx_attn_forward_workspace: null size pointer");
   const int rows = d->heads / d->kv_heads * d->q_len;
-  *bytes = fwd_floats(d, plan_of(d->batch * d->kv_heads, rows, d->k_len, d->causal)) * sizeof(float);
+  *bytes = fwd_floats(d, plan_of(d->batch * d->kv_heads, rows, d->k_len, d->causal, d->heads / d->kv_heads)) * sizeof(float);
   return FDX_OK;
 }
 
@@ -977,7 +982,7 @@ extern "C" int fdx_attn_backward_workspace(const fdx_attn_desc* d, size_t* bytes
   if (const char* why = check(d)) return fail(nullptr, FDX_E_ARG, "fdx_attn_backward_workspace: %s", why);
   if (!bytes) return fail(nullptr, FDX_E_ARG, "fdx_attn_backward_workspace: null size pointer");
   const int rows = d->heads / d->kv_heads * d->q_len, nb = d->batch * d->kv_heads;
-  *bytes = (delta_floats(d) + std::max(dq_floats(d, plan_of(nb, rows, d->k_len, d->causal)), dkv_floats(d, plan_of(nb, d->k_len, rows, d->causal)))) * sizeof(float);
+  *bytes = (delta_floats(d) + std::max(dq_floats(d, plan_of(nb, rows, d->k_len, d->causal, d->heads / d->kv_heads)), dkv_floats(d, plan_of(nb, d->k_len, rows, d->causal, 1)))) * sizeof(float);
   return FDX_OK;
 }
 
@@ -992,7 +997,7 @@ extern "C" int fdx_attn_forward(fdx_handle h, const fdx_attn_desc* d, const fdx_
     if (const char* why = check(d, x.t, x.need)) return fail(h, FDX_E_ARG, "fdx_attn_forward: %s", why);
   if (!lse) return fail(h, FDX_E_ARG, "fdx_attn_forward: null lse");
   AttnArgs a = args_of(d);
-  const Plan p = plan_of(a.B * a.Hkv, a.R, a.Tk, a.causal);
+  const Plan p = plan_of(a.B * a.Hkv, a.R, a.Tk, a.causal, a.G);
   if (bytes < fwd_floats(d, p) * sizeof(float) || (p.splits > 1 && !workspace))
     return fail(h, FDX_E_ARG, "fdx_attn_forward: workspace of %zu bytes, %zu needed", bytes, fwd_floats(d, p) * sizeof(float));
   a.q = q->data; a.k = k ? k->data : nullptr; a.v = v ? v->data : nullptr; a.o = out->data;
@@ -1016,7 +1021,7 @@ extern "C" int fdx_attn_backward(fdx_handle h, const fdx_attn_desc* d, const fdx
     if (const char* why = check(d, x.t, x.need)) return fail(h, FDX_E_ARG, "fdx_attn_backward: %s", why);
   if (rows && !lse) return fail(h, FDX_E_ARG, "fdx_attn_backward: null lse");
   AttnArgs a = args_of(d);
-  const Plan pq = plan_of(a.B * a.Hkv, a.R, a.Tk, a.causal), pk = plan_of(a.B * a.Hkv, a.Tk, a.R, a.causal);
+  const Plan pq = plan_of(a.B * a.Hkv, a.R, a.Tk, a.causal, a.G), pk = plan_of(a.B * a.Hkv, a.Tk, a.R, a.causal, 1);
   const size_t need = (delta_floats(d) + std::max(dq_floats(d, pq), dkv_floats(d, pk))) * sizeof(float);
   if (bytes < need || (need && !workspace)) return fail(h, FDX_E_ARG, "fdx_attn_backward: workspace of %zu bytes, %zu needed", bytes, need);
   const auto data = [](const fdx_bht* t) { return t ? t->data : nullptr; };
