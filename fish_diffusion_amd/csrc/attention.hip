@@ -55,7 +55,7 @@ __device__ inline float half_sum(float x) {
 
 // workgroup -> (batch and kv head, tile, split).  Workgroups go to the 8 XCDs in turn: where the heads divide, all tiles of a head run on one
 // XCD and find its K / V in that XCD's L2.  Causal tiles start in the order of their length, the G heads' longest first: the grid then has G times
-// ceil(tiles / G) places and those past the last tile end at once (2 x 16 / 4 heads x 4096 x 128: forward 212 -> MEASURED us against head after head).
+// ceil(tiles / G) places and those past the last tile end at once (2 x 16 / 4 heads x 4096 x 128: forward 212 -> 169 us, dq 346 -> 280 us against head after head).
 __device__ inline void decode(const AttnArgs& a, int G, int& bh, int& tile, int& split) {
   const int nb = a.B * a.Hkv, per = a.tiles * a.splits, i = blockIdx.x;
   int j;
@@ -684,10 +684,11 @@ __global__ __launch_bounds__(256, (waves_of<T, DH>())) void k_attn_dkv(AttnArgs 
   constexpr int KS = Elem<T>::KS, WR = 4 / WN, TR = RT * WR, NS = DH / KS, MT = DH / 32, NU = RT / 32, NP = 32 / KS;
   constexpr int kTile = TR * Tl::CPR, kMerge = WR > 1 ? WR * 32 * DH / 4 : 0;
   static_assert(TR % 64 == 0 || TR == 32, "rows voted on 64 at a time");
-  constexpr int S = stages_of(32 * kTile);
+  constexpr bool PARK = parked<T, DH>();
+  // (64 rows in one stage beat 32 in two where v is parked: 368 against 399 us, bf16, head size 128, 2 x 16 / 4 x 4096 causal)
+  constexpr int S = stages_of(32 * kTile + (PARK ? WN * NS * 1024 : 0));
   __shared__ __attribute__((aligned(1024))) uint4 smem[2 * S * kTile > kMerge ? 2 * S * kTile : kMerge];   // S stages of q and do
   __shared__ __attribute__((aligned(16))) float rowL[2][TR], rowD[2][TR];
-  constexpr bool PARK = parked<T, DH>();
   __shared__ uint4 own[PARK ? WN * NS * 64 : 1];
   int bh, tile, split;
   decode(a, 1, bh, tile, split);
@@ -960,7 +961,7 @@ template <typename T, int DH> struct RunBwd {
     if (e == hipSuccess && a.Tk > 0) {   // (reuses the partial sums' memory: ordered by the stream)
       a.tiles = pk.tiles; a.splits = pk.splits;
       const unsigned grid = (unsigned)((long)a.B * a.Hkv * pk.tiles * pk.splits);
-      e = pk.narrow ? launch(k_attn_dkv<T, DH, 1, 32>, grid, 256, a, s) : launch(k_attn_dkv<T, DH, 4, (DH * sizeof(T) >= 256 ? 32 : 64)>, grid, 256, a, s);
+      e = pk.narrow ? launch(k_attn_dkv<T, DH, 1, 32>, grid, 256, a, s) : launch(k_attn_dkv<T, DH, 4, (sizeof(T) == 4 && DH > 32 ? 32 : 64)>, grid, 256, a, s);
       if (e == hipSuccess && pk.splits > 1)
         e = launch(k_attn_join_dkv<T>, (unsigned)(((long)a.B * a.Hkv * a.Tk * (a.D / 4) * 2 + 255) / 256), 256, a, s);
     }
