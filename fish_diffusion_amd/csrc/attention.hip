@@ -77,9 +77,12 @@ __device__ inline int key_end(const AttnArgs& a, int r0, int r1) {
 // other workgroup's products cover the loads)
 constexpr int stages_of(int bytes) { return 2 * bytes <= 80 * 1024 ? 2 : 1; }
 
-// which of a step's TK rows exist and are not masked, in every wave: loaded one step before it is needed
+// which of a step's TK rows exist and are not masked, in every wave: loaded one step before it is needed.  (Picked by comparison: an array indexed by
+// a lane's value goes to LDS, addressed through the dispatch packet in host memory -- 12 us per launch.)
+__device__ inline bool bit_of(const unsigned long long* bits, int n, int row) { return ((n > 1 && row >= 64 ? bits[n > 1 ? 1 : 0] : bits[0]) >> (row & 63)) & 1; }
 template <int TK> struct RowBits {
   static constexpr int N = (TK + 63) / 64;
+  static_assert(N <= 2, "two words");
   unsigned char m[N];
   unsigned long long bits[N];
   __device__ inline void load(const uint8_t* mask, int first, int end, int lane) {
@@ -93,7 +96,12 @@ template <int TK> struct RowBits {
 #pragma unroll
     for (int i = 0; i < N; ++i) bits[i] = __ballot(m[i] == 0);
   }
-  __device__ inline bool has(int row) const { return (bits[N == 1 ? 0 : row >> 6] >> (row & 63)) & 1; }
+  __device__ inline bool has(int row) const { return bit_of(bits, N, row); }
+  // KT rows from wk * KT on
+  template <int KT> __device__ inline unsigned long long part(int wk) const {
+    if constexpr (N == 1 && KT >= 64) return bits[0];
+    else return ((N > 1 && wk * KT >= 64 ? bits[N - 1] : bits[0]) >> (wk * KT % 64)) & (~0ull >> (64 - KT));
+  }
   __device__ inline bool all() const {
     unsigned long long o = ~0ull;
 #pragma unroll
@@ -238,8 +246,7 @@ __global__ __launch_bounds__(256, (waves_of<T, DH>())) void k_attn_fwd(AttnArgs 
     landed();
     const unsigned row = opaque(row0 + stage * 2 * kTile * 16), col = opaque(col0 + stage * 2 * kTile * 16);   // K; V: kTile rows' bytes behind
     constexpr int V0 = TK;
-    unsigned long long bits = rb.bits[wk * KT / 64];
-    if constexpr (KT == 32) bits = (bits >> (wk * KT % 64)) & 0xffffffffull;
+    const unsigned long long bits = rb.template part<KT>(wk);
     if constexpr (S == 2) stage ^= 1;
     if (st + a.splits < steps) {
       rb.vote();
@@ -496,8 +503,7 @@ __global__ __launch_bounds__(256, (waves_of<T, DH>())) void k_attn_dq(AttnArgs a
     landed();
     const unsigned row = opaque(row0 + stage * 2 * kTile * 16), col = opaque(col0 + stage * 2 * kTile * 16);   // K; V: kTile rows' bytes behind
     constexpr int V0 = TK;
-    unsigned long long bits = rb.bits[wk * KT / 64];
-    if constexpr (KT == 32) bits = (bits >> (wk * KT % 64)) & 0xffffffffull;
+    const unsigned long long bits = rb.template part<KT>(wk);
     if constexpr (S == 2) stage ^= 1;
     if (st + a.splits < steps) {
       rb.vote();
@@ -750,7 +756,7 @@ __global__ __launch_bounds__(256, (waves_of<T, DH>())) void k_attn_dkv(AttnArgs 
         rowD[stage][64 * i + lane] = nL[i] == -inf() ? 0.f : nD[i];
       }
     }
-    auto has = [&](int row) { return (live[NB == 1 ? 0 : row >> 6] >> (row & 63)) & 1; };
+    auto has = [&](int row) { return bit_of(live, NB, row); };
     uint4* const to = smem + stage * 2 * kTile;
     bool all = a.D == DH;
 #pragma unroll
