@@ -871,14 +871,17 @@ __global__ __launch_bounds__(256, (waves_of<T, DH>())) void k_attn_dkv(AttnArgs 
 // ---------------------------------------------------------------------------------------------------------------- launches
 namespace {
 
-// How a pass is cut.  Four waves x 32 rows share every staged tile where that alone gives two workgroups per CU; below, 32-row workgroups
-// whose waves share the keys; and while even those leave CUs empty the other axis is split over workgroups and joined.  512 workgroups are resident;
-// causal tiles differ in length by up to all of it, and twice as many workgroups as are resident, long ones first, even that out.
+// How a pass is cut.  Four waves x 32 rows share every staged tile where that gives more than one workgroup per CU (1024 tiles of 32 rows); below, 32-row
+// workgroups whose waves share the keys.  Forward, 128-row / 32-row form, us: fp32 head size 64, 86 rows x 8 heads 13.1 / 7.7; bf16 64: 256 tiles of 32 rows
+// 13.3 / 6.0, 864: 35.2 / 24.2, 1024: 48.1 / 42.6, 1728: 26.9 / 45.5.
+// Causal tiles stop there at half as many: a 32-row workgroup's waves have few keys each in the short ones (1024: forward 56.6 / 55.5, dk and dv 389 / 434).
+// While even those leave CUs empty the other axis is split over workgroups and joined.  512 workgroups are resident; causal tiles differ in length by up to
+// all of it, and twice as many workgroups as are resident, long ones first, even that out (dk / dv, 2 x 4 heads x 4096 x 128: 1094 us in 256 workgroups, 408 in 1024).
 struct Plan { int narrow, tiles, splits; };   // narrow: 32 rows per workgroup
 Plan plan_of(int nb, int rows, int across, bool causal, int G) {   // G: heads in the rows
   Plan p;
   const long n32 = (long)nb * ((rows + 31) / 32);
-  p.narrow = n32 <= 512;
+  p.narrow = n32 <= (causal ? 512 : 1024);
   p.tiles = p.narrow ? (rows + 31) / 32 : (rows + 127) / 128;
   const long base = std::max<long>(1, (long)nb * p.tiles), want = causal ? 1024 : 512;
   const int steps = p.narrow ? (across + 127) / 128 : (across + 63) / 64;

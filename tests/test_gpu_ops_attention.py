@@ -128,8 +128,10 @@ def test_attention_and_gradients(t, shape, causal, kind):
     check(both(q, k, v, do, mask, causal), want, tol, ALL)
 
 
-# the 128-row form (more than 512 tiles of 32 rows), its split form, and both for the keys of dk / dv
+# the 128-row form (more than 1024 tiles of 32 rows), its split form, and both for the keys of dk / dv
 @pytest.mark.parametrize("t,shape,causal", [
+    ("f32", (8, 16, 16, 290, 300, 64), False), ("bf16", (8, 16, 16, 290, 300, 64), True), ("f16", (8, 16, 4, 290, 310, 128), True), ("f32", (9, 20, 4, 270, 270, 128), True),
+    ("bf16", (1, 1, 1, 34000, 300, 32), False), ("f32", (1, 1, 1, 300, 34000, 32), False), ("bf16", (1, 4, 1, 8500, 260, 128), True), ("f16", (40, 16, 16, 60, 60, 40), True),
     ("f32", (8, 8, 8, 300, 300, 64), False), ("bf16", (8, 8, 8, 300, 300, 64), True), ("f16", (8, 8, 4, 290, 310, 128), True),
     ("f32", (2, 40, 8, 270, 333, 128), True), ("bf16", (1, 1, 1, 20000, 300, 32), False), ("f32", (1, 1, 1, 300, 20000, 32), False),
     ("f16", (1, 2, 2, 1100, 9000, 64), False), ("bf16", (1, 4, 1, 4400, 260, 128), True)], ids=str)
