@@ -189,7 +189,7 @@ template <> struct PShift<f16_t> { static constexpr float log2 = 11.f, back = 0x
 
 // ---------------------------------------------------------------------------------------------------------------- forward
 // WQ waves take 32 rows each, the other factor of the 4 waves (WK) shares those rows and takes KT keys each of every step; their
-// (max, sum, O) meet in LDS at the end.  Online softmax: running maximum m of the raw scores, P = exp2(c s - c m).
+// (reference, sum, O) meet in LDS at the end.  Online softmax: P = exp2(c s - m) with m a reference that follows the row's maximum (below).
 template <typename T, int DH, int WQ, int KT>
 __global__ __launch_bounds__(256, (waves_of<T, DH>())) void k_attn_fwd(AttnArgs a) {
   typedef Tile<T, DH> Tl;
@@ -244,7 +244,7 @@ __global__ __launch_bounds__(256, (waves_of<T, DH>())) void k_attn_fwd(AttnArgs 
       rb.load(mask, (st + a.splits) * TK, a.Tk, lane);
     }
     landed();
-    const unsigned row = opaque(row0 + stage * 2 * kTile * 16), col = opaque(col0 + stage * 2 * kTile * 16);   // K; V: kTile rows' bytes behind
+    const unsigned row = opaque(row0 + stage * 2 * kTile * 16), col = opaque(col0 + stage * 2 * kTile * 16);   // K; V: TK rows behind
     constexpr int V0 = TK;
     const unsigned long long bits = rb.template part<KT>(wk);
     if constexpr (S == 2) stage ^= 1;
@@ -501,7 +501,7 @@ __global__ __launch_bounds__(256, (waves_of<T, DH>())) void k_attn_dq(AttnArgs a
       rb.load(mask, (st + a.splits) * TK, a.Tk, lane);
     }
     landed();
-    const unsigned row = opaque(row0 + stage * 2 * kTile * 16), col = opaque(col0 + stage * 2 * kTile * 16);   // K; V: kTile rows' bytes behind
+    const unsigned row = opaque(row0 + stage * 2 * kTile * 16), col = opaque(col0 + stage * 2 * kTile * 16);   // K; V: TK rows behind
     constexpr int V0 = TK;
     const unsigned long long bits = rb.template part<KT>(wk);
     if constexpr (S == 2) stage ^= 1;
@@ -901,12 +901,17 @@ const char* check(const fdx_attn_desc* d) {
   if (!(d->scale > 0.f) || !std::isfinite(d->scale)) return "scale must be positive and finite";
   const long R = (long)(d->heads / d->kv_heads) * d->q_len, nb = (long)d->batch * d->kv_heads;
   if (R > INT_MAX / 2 || d->k_len > INT_MAX / 2) return "too many rows for one key / value head";
-  if (nb * ((R + 31) / 32 + d->heads) > INT_MAX / 64 || nb * (((long)d->k_len + 31) / 32) > INT_MAX / 64) return "too many tiles for one launch";
+  constexpr long most = (1L << 24) - 1;   // workgroups of 256 threads in one launch
+  if (nb * ((R + 31) / 32 + d->heads) > most || nb * (((long)d->k_len + 31) / 32) > most) return "too many tiles for one launch";
   return nullptr;
 }
 
-const char* check(const fdx_attn_desc* d, const fdx_bht* t, bool required) {
-  if (!t || !t->data) return required ? "null tensor" : nullptr;
+struct Checked { const fdx_bht* t; bool need; int heads, rows; };   // heads, rows: of a tensor that is written, else 0
+const char* check(const fdx_attn_desc* d, const Checked& x) {
+  const fdx_bht* const t = x.t;
+  if (!t || !t->data) return x.need ? "null tensor" : nullptr;
+  if (t->b < 0 || t->h < 0 || t->t < 0) return "strides must not be negative";
+  if (x.heads && ((d->batch > 1 && !t->b) || (x.heads > 1 && !t->h) || (x.rows > 1 && !t->t))) return "results must not overlap themselves (stride 0)";
   const int vec = d->dtype == DT_F32 ? 4 : 8;
   if ((reinterpret_cast<uintptr_t>(t->data) & 15) || t->b % vec || t->h % vec || t->t % vec) return "tensors must be 16-byte aligned, strides whole 16 bytes";
   return nullptr;
@@ -1002,14 +1007,13 @@ extern "C" int fdx_attn_forward(fdx_handle h, const fdx_attn_desc* d, const fdx_
   if (const char* why = check(d)) return fail(h, FDX_E_ARG, "fdx_attn_forward: %s", why);
   if (d->batch == 0 || d->q_len == 0) return FDX_OK;
   const bool keys = d->k_len > 0;
-  const struct { const fdx_bht* t; bool need; } all[] = {{q, true}, {k, keys}, {v, keys}, {out, true}};
-  for (const auto& x : all)
-    if (const char* why = check(d, x.t, x.need)) return fail(h, FDX_E_ARG, "fdx_attn_forward: %s", why);
+  for (const Checked& x : {Checked{q, true, 0, 0}, {k, keys, 0, 0}, {v, keys, 0, 0}, {out, true, d->heads, d->q_len}})
+    if (const char* why = check(d, x)) return fail(h, FDX_E_ARG, "fdx_attn_forward: %s", why);
   if (!lse) return fail(h, FDX_E_ARG, "fdx_attn_forward: null lse");
   AttnArgs a = args_of(d);
   const Plan p = plan_of(a.B * a.Hkv, a.R, a.Tk, a.causal, a.G);
-  if (bytes < fwd_floats(d, p) * sizeof(float) || (p.splits > 1 && !workspace))
-    return fail(h, FDX_E_ARG, "fdx_attn_forward: workspace of %zu bytes, %zu needed", bytes, fwd_floats(d, p) * sizeof(float));
+  if (bytes < fwd_floats(d, p) * sizeof(float) || (p.splits > 1 && !workspace) || (reinterpret_cast<uintptr_t>(workspace) & 15))
+    return fail(h, FDX_E_ARG, "fdx_attn_forward: workspace of %zu bytes, %zu needed (16-byte aligned)", bytes, fwd_floats(d, p) * sizeof(float));
   a.q = q->data; a.k = k ? k->data : nullptr; a.v = v ? v->data : nullptr; a.o = out->data;
   a.sq = str_of(q); a.sk = str_of(k); a.sv = str_of(v); a.so = str_of(out);
   a.mask = key_mask; a.lse = lse; a.part = static_cast<float*>(workspace);
@@ -1026,14 +1030,15 @@ extern "C" int fdx_attn_backward(fdx_handle h, const fdx_attn_desc* d, const fdx
   if (const char* why = check(d)) return fail(h, FDX_E_ARG, "fdx_attn_backward: %s", why);
   if (d->batch == 0 || (d->q_len == 0 && d->k_len == 0)) return FDX_OK;
   const bool rows = d->q_len > 0, keys = d->k_len > 0;
-  const struct { const fdx_bht* t; bool need; } all[] = {{grad_out, rows}, {q, rows}, {out, rows}, {dq, rows}, {k, keys}, {v, keys}, {dk, keys}, {dv, keys}};
-  for (const auto& x : all)
-    if (const char* why = check(d, x.t, x.need)) return fail(h, FDX_E_ARG, "fdx_attn_backward: %s", why);
+  for (const Checked& x : {Checked{grad_out, rows, 0, 0}, {q, rows, 0, 0}, {out, rows, 0, 0}, {dq, rows, d->heads, d->q_len}, {k, keys, 0, 0}, {v, keys, 0, 0},
+                           {dk, keys, d->kv_heads, d->k_len}, {dv, keys, d->kv_heads, d->k_len}})
+    if (const char* why = check(d, x)) return fail(h, FDX_E_ARG, "fdx_attn_backward: %s", why);
   if (rows && !lse) return fail(h, FDX_E_ARG, "fdx_attn_backward: null lse");
   AttnArgs a = args_of(d);
   const Plan pq = plan_of(a.B * a.Hkv, a.R, a.Tk, a.causal, a.G), pk = plan_of(a.B * a.Hkv, a.Tk, a.R, a.causal, 1);
   const size_t need = (delta_floats(d) + std::max(dq_floats(d, pq), dkv_floats(d, pk))) * sizeof(float);
-  if (bytes < need || (need && !workspace)) return fail(h, FDX_E_ARG, "fdx_attn_backward: workspace of %zu bytes, %zu needed", bytes, need);
+  if (bytes < need || (need && !workspace) || (reinterpret_cast<uintptr_t>(workspace) & 15))
+    return fail(h, FDX_E_ARG, "fdx_attn_backward: workspace of %zu bytes, %zu needed (16-byte aligned)", bytes, need);
   const auto data = [](const fdx_bht* t) { return t ? t->data : nullptr; };
   a.q = data(q); a.k = data(k); a.v = data(v); a.go = data(grad_out); a.o = data(out);
   a.dq = data(dq); a.dk = data(dk); a.dv = data(dv);

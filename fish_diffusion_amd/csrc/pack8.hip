@@ -539,7 +539,8 @@ extern "C" int fdx_linear8_weight_grad(fdx_handle h, int dtype, const void* dy, 
   const char* why = check(dtype, rows, out_features);
   if (!why) why = check(grad_dtype, rows, in_features);
   const long tiles = (long)((out_features + 127) / 128) * ((in_features + 127) / 128);
-  if (!why && (tiles > INT_MAX / 64 || (long)out_features * in_features / 1024 > INT_MAX / 2)) why = "too many tiles for one launch";
+  constexpr long most = (1L << 24) - 1;   // workgroups of 256 threads in one launch
+  if (!why && (tiles > most / 64 || (long)out_features * in_features / 1024 + out_features / 32 + 2 > most)) why = "too many tiles for one launch";
   if (!why && (!dw || (rows > 0 && (!dy || !codes || !exps)))) why = "null tensor";
   if (why) return fail(h, FDX_E_ARG, "fdx_linear8_weight_grad: %s", why);
   const Cut8 c = wgrad_cut(rows, out_features, in_features);

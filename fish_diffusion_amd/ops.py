@@ -516,14 +516,16 @@ class _Linear8(torch.autograd.Function):
     def forward(ctx, x, weight, bias):
         ctx.save_for_backward(*pack8(x), weight)
         ctx.has_bias = bias is not None
-        return torch.nn.functional.linear(x, weight, bias)
+        with torch.autocast(x.device.type, enabled=False):   # the result has x's type, as the gradient that comes back
+            return torch.nn.functional.linear(x, weight, bias)
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dy):
         codes, exps, weight = ctx.saved_tensors
         need_x, need_w, need_b = ctx.needs_input_grad
-        dx = torch.matmul(dy, weight) if need_x else None
+        with torch.autocast(dy.device.type, enabled=False):
+            dx = torch.matmul(dy, weight) if need_x else None
         dw, db = linear8_weight_grad(dy, Packed8(codes, exps), ctx.has_bias) if need_w or need_b else (None, None)
         return dx, dw, db
 

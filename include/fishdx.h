@@ -416,7 +416,8 @@ int fdx_repeat_expand(fdx_handle h, const float* src, long rows, int S, int T, f
  * *_workspace functions give (16-byte aligned; one per call in flight).  No atomics: the same inputs give the same bits.
  * ---------------------------------------------------------------------------------------------- */
 enum { FDX_F32 = 0, FDX_BF16 = 1, FDX_F16 = 2 };
-/* A [batch][heads][length][channels] tensor, channels contiguous, the other strides in elements.  data 16-byte aligned, strides whole 16 bytes. */
+/* A [batch][heads][length][channels] tensor, channels contiguous, the other strides in elements.  data 16-byte aligned, strides whole 16 bytes and not
+ * negative; 0 repeats (not in results). */
 typedef struct { void* data; long long b, h, t; } fdx_bht;
 typedef struct fdx_attn_desc {
   int dtype;                 /* FDX_F32 | FDX_BF16 | FDX_F16: q, k, v, out and their gradients; scores and sums are fp32 */

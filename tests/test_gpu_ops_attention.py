@@ -307,3 +307,35 @@ def test_refusals_on_the_device():
     assert lib.fdx_attn_forward(h.h, C.byref(desc), b(q, 4), b(k), b(v), None, b(out), _lib.ptr(lse), None, 0, st) == -1
     assert lib.fdx_attn_backward(h.h, C.byref(desc), b(do), b(q), b(k), b(v), b(out), _lib.ptr(lse), None, b(q), b(k), b(v), None, 0, st) == -1
     assert b"workspace" in lib.fdx_last_error(h.h)
+
+
+def test_c_entries_refuse_strides_and_workspaces():
+    import ctypes as C
+    from fish_diffusion_amd import _lib
+    q, k, v, do = inputs(torch.float32, 2, 2, 2, 8, 8, 32)
+    out, lse, ws = torch.empty_like(q), torch.empty(2, 2, 8, device="cuda"), torch.empty(1 << 16, dtype=torch.uint8, device="cuda")
+    desc, h, lib, st = _lib.AttnDesc(0, 2, 2, 2, 8, 8, 32, 0, 1.0), _lib.Handle.shared(q.device), _lib.lib(), _lib.stream_ptr(q.device)
+
+    def bht(x, **strides):
+        s = dict(b=x.stride(0), h=x.stride(1), t=x.stride(2))
+        s.update(strides)
+        return C.byref(_lib.Bht(x.data_ptr(), s["b"], s["h"], s["t"]))
+
+    def forward(q=bht(q), out=bht(out), at=0):
+        return lib.fdx_attn_forward(h.h, C.byref(desc), q, bht(k), bht(v), None, out, _lib.ptr(lse), ws.data_ptr() + at, ws.numel() - at, st)
+
+    def backward(dk=bht(do), at=0):
+        return lib.fdx_attn_backward(h.h, C.byref(desc), bht(do), bht(q), bht(k), bht(v), bht(out), _lib.ptr(lse), None, bht(do), dk, bht(do), ws.data_ptr() + at,
+                                     ws.numel() - at, st)
+
+    for bad in (dict(b=-512), dict(h=-256), dict(t=-32)):
+        assert forward(q=bht(q, **bad)) == -1 and b"negative" in lib.fdx_last_error(h.h)
+        assert backward(dk=bht(k, **bad)) == -1
+    for bad in (dict(b=0), dict(h=0), dict(t=0)):
+        assert forward(out=bht(out, **bad)) == -1 and b"overlap" in lib.fdx_last_error(h.h)
+        assert backward(dk=bht(k, **bad)) == -1
+    assert forward(at=4) == -1 and backward(at=4) == -1 and b"aligned" in lib.fdx_last_error(h.h)
+    assert forward(q=bht(q, h=0)) == 0          # a repeated head is an input like any other
+    torch.cuda.synchronize()
+    want = torch.softmax((q[:, :1].double() @ k.double().transpose(-1, -2)), -1) @ v.double()
+    assert (out.double() - want).abs().max() < 1e-3     # scores of up to 60 in sums of 32 products: 33 * 60 * 2^-24 = 1.2e-4 of P, |v| <= 4

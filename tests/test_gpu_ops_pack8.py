@@ -208,3 +208,15 @@ def test_finite_values_stay_finite():
             y = fda.unpack8(p, o)
             if torch.finfo(o).max >= torch.finfo(t).max or o == torch.float16:
                 assert torch.isfinite(y).all() and (y[0] > 0).all() and (y[1] < 0).all()
+
+
+def test_linear_under_autocast_keeps_its_type():
+    import fish_diffusion_amd as fda
+    x, w, b = (make(torch.float32, *s, seed=i).requires_grad_() for i, s in enumerate(((9, 64), (40, 64), (40,))))
+    dy = make(torch.float32, 9, 40, seed=5)
+    want = torch.autograd.grad(fda.linear8(x, w, b), (x, w, b), dy)
+    with torch.autocast("cuda", dtype=torch.bfloat16):
+        y = fda.linear8(x, w, b)
+        got = torch.autograd.grad(y, (x, w, b), dy)
+    assert y.dtype == torch.float32 and torch.equal(y, fda.linear8(x, w, b))
+    assert all(torch.equal(g, t) for g, t in zip(got, want))

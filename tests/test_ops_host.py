@@ -45,7 +45,8 @@ def test_workspace_sizes_and_bad_descriptors(lib_built):
     assert lib.fdx_attn_backward_workspace(C.byref(d), C.byref(n)) == 0 and n.value > 0
     assert lib.fdx_attn_forward_workspace(C.byref(d), None) == -1
     for bad in (dict(dtype=3), dict(heads=0), dict(kv_heads=5), dict(head_dim=12), dict(head_dim=256), dict(q_len=-1), dict(scale=0.0),
-                dict(scale=float("inf")), dict(heads=1 << 20, kv_heads=1, q_len=1 << 20)):
+                dict(scale=float("inf")), dict(heads=1 << 20, kv_heads=1, q_len=1 << 20),
+                dict(batch=1 << 23, heads=1, kv_heads=1)):
         d = _lib.AttnDesc(1, 1, 32, 8, 1, 8192, 128, 0, 1.0)
         for k, v in bad.items():
             setattr(d, k, v)
