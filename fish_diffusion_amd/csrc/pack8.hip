@@ -162,9 +162,14 @@ template <typename T, bool GRAD> __global__ __launch_bounds__(256) void k_unpack
 }
 
 // ---------------------------------------------------------------------------------------------------------------- weight gradient
-// A workgroup computes a tile of dW over its share of the rows n, 64 * MO output by 128 input channels, in four waves of (32 * MO) x 64.  KT rows of dy
-// (in bf16 planes) and of x8 (decoded) stand in LDS, two stages, both read as column fragments by transposing reads: MO + 2 fragments feed 2 * MO matrix
-// instructions, so at MO = 4 the LDS delivers 3/4 of what it can while they run.  bf16 dy goes straight to LDS; the wider types pass registers to be split.
+// A workgroup computes a tile of dW over its share of the rows n: 256 x 128 channels in two halves of four waves, each with all of the tile
+// ((32 MO) x (32 NI) a wave) over every other step of rows.  The halves' sums meet in LDS at the end, so a CU full of accumulators leaves one partial tile
+// instead of two (two independent workgroups of four waves: 59 + 14 us with the join against 55 + 8; fp32, 6888 rows, 2048 x 512).
+// KT rows of dy (in bf16 planes) and of x8 (decoded) stand in LDS, two stages per half, both read as column fragments by transposing reads: MO + NI fragments
+// feed MO * NI matrix instructions.  bf16 dy goes straight to LDS, and the 256 are its channels: decoding x is all the arithmetic (per product least so).
+// The wider types pass registers to be split, the 256 are x's: splitting is the arithmetic then.
+// 128 x 128 tiles take what is odd.  Bound by the matrix instructions with the conversions between them (fp32: 770 TFLOP/s of bf16 products at 6888 rows) and,
+// for bf16 dy, the LDS (per 16 rows 24 KB of reads and 12 of writes for 256 cycles of matrix instructions).
 // Rows are shared out over `splits` workgroups (an XCD takes whole shares: dy and x8 stay in its L2 for all tiles) whose fp32 partial tiles a second
 // launch joins in order.  db is summed from what is staged, each tile column taking every ti-th step.
 struct WgradArgs {
@@ -173,7 +178,7 @@ struct WgradArgs {
   const uint8_t* exps;
   float *part, *part_b;   // [splits][O][I], [splits][ti][O]
   long N, rows;           // rows per split: a multiple of 32
-  int O, I, G, to, ti, splits, bias, vec_dy, vec_x;
+  int O, I, G, to, ti, splits, bias;
 };
 
 template <typename T> struct Planes { static constexpr int n = 3; };
@@ -196,101 +201,117 @@ __device__ inline uint4 decode8(uint2 c, float scale) {
   return w;
 }
 
-template <typename T, int MO>
-__global__ __launch_bounds__(256, 2) void k_linear8_wgrad(WgradArgs a) {
+template <typename T, int MO, int NI, bool VEC>
+__global__ __launch_bounds__(512, 2) void k_linear8_wgrad(WgradArgs a) {
   typedef Tile<bf16_t, 128> Tl;
   typedef Elem<bf16_t>::frag frag;
-  constexpr int P = Planes<T>::n, KT = P == 1 ? 32 : 16, NO = MO / 2;   // NO: 128-channel tiles of dy
-  constexpr int kY = KT * 16, kX = KT * 16, kStage = P * NO * kY + kX;   // in 16-byte units
-  __shared__ __attribute__((aligned(1024))) uint4 smem[2 * kStage];
+  constexpr int P = Planes<T>::n, KT = P == 1 ? 32 : 16, NO = MO / 2, NX = NI / 2;   // NO, NX: 128-channel tiles of dy and x
+  constexpr int kY = KT * 16, kStage = (P * NO + NX) * kY;   // in 16-byte units; kY: one tile
+  constexpr int kSum = 256 * MO * NI * 4;   // one half's accumulators
+  __shared__ __attribute__((aligned(1024))) uint4 smem[4 * kStage > kSum ? 4 * kStage : kSum];
   const int per = a.to * a.ti;
   int split, j;
   if (a.splits % 8 == 0) { split = (blockIdx.x & 7) + 8 * ((blockIdx.x >> 3) / per); j = (blockIdx.x >> 3) % per; }
   else { split = blockIdx.x / per; j = blockIdx.x % per; }
-  const int jo = j / a.ti, ji = j % a.ti, o0 = jo * 128 * NO, i0 = ji * 128;
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wo = wave >> 1, wi = wave & 1;
+  const int jo = j / a.ti, ji = j % a.ti, o0 = jo * 128 * NO, i0 = ji * 128 * NX;
+  const int lane = threadIdx.x & 63, wave = (threadIdx.x >> 6) & 3, wo = wave >> 1, wi = wave & 1, tid = threadIdx.x & 255;
+  const int half = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 8);
+  uint4* const own = smem + half * 2 * kStage;
   // staging of x: 8 columns of XR rows; of dy (through registers): 8 columns of YR rows
-  constexpr int XR = KT / 16, YC = 16 * NO, YR = KT * YC / 256;
-  const int xc = threadIdx.x & 15, xr = threadIdx.x >> 4, yc = threadIdx.x % YC, yr = threadIdx.x / YC;
+  constexpr int XC = 16 * NX, XR = KT * XC / 256, YC = 16 * NO, YR = KT * YC / 256;
+  const int xc = tid % XC, xr = tid / XC, yc = tid % YC, yr = tid / YC;
   const int ic = i0 + 8 * xc, in = a.I - ic, oc = o0 + 8 * yc, on = a.O - oc;
   float db[8] = {0, 0, 0, 0, 0, 0, 0, 0};
-  f32x16 acc[MO][2];
+  f32x16 acc[MO][NI];
 #pragma unroll
   for (int m = 0; m < MO; ++m)
 #pragma unroll
-    for (int n = 0; n < 2; ++n) acc[m][n] = f32x16{0};
+    for (int n = 0; n < NI; ++n) acc[m][n] = f32x16{0};
   const long nb = (long)split * a.rows, ne = min(a.N, nb + a.rows);
-  // wave wo's channels: MO == 4: its own 128-channel tile, MO == 2: half of the one
-  const unsigned coly = lds_of(smem) + (Tl::col_base(lane) ^ (MO == 2 ? 128 * wo : 0)) + (MO == 4 ? wo * P * kY * 16 : 0);
-  const unsigned colx = lds_of(smem) + P * NO * kY * 16 + (Tl::col_base(lane) ^ (128 * wi));
+  // wave wo's channels: MO == 4: its own 128-channel tile, MO == 2: half of the one (wi, NI: the same for x)
+  const unsigned coly = lds_of(own) + (Tl::col_base(lane) ^ (MO == 2 ? 128 * wo : 0)) + (MO == 4 ? wo * P * kY * 16 : 0);
+  const unsigned colx = lds_of(own) + P * NO * kY * 16 + (Tl::col_base(lane) ^ (NI == 2 ? 128 * wi : 0)) + (NI == 4 ? wi * kY * 16 : 0);
 
-  uint2 xcode[XR];
-  int xexp[XR];
-  float y[P == 1 ? 1 : YR][8];
-  auto load_x = [&](long n0) {
+  // Registers of two steps ahead.  They hold what was loaded as it was loaded: any instruction on it here -- a conversion, the masking of a byte --
+  // would wait for the load in front of the products instead of behind them.  Rows past the last one are read as the last one and made zeros when they
+  // are used; columns past the last one are never stored.
+  typedef T t8 __attribute__((ext_vector_type(8)));
+  uint2 xcode[2][XR];
+  int xexp[2][XR];
+  t8 y[2][YR];
+  const int icv = in > 0 ? ic : 0, ocv = on > 0 ? oc : 0;
+  auto load_x = [&](long n0, int set) {
+    const int last = (int)min((long)KT, ne - n0) - 1;
+    const int8_t* const p = a.codes + n0 * a.I + icv;
+    const uint8_t* const pe = a.exps + n0 * a.G + (icv >> 5);
+#pragma unroll
+    for (int h = 0; h < XR; ++h) xexp[set][h] = pe[(long)min(xr + (256 / XC) * h, last) * a.G];
 #pragma unroll
     for (int h = 0; h < XR; ++h) {
-      const long n = n0 + xr + 16 * h;
-      const bool ok = n < ne && in > 0;
-      const int8_t* const p = a.codes + n * a.I + ic;
-      xcode[h] = uint2{0, 0};
-      xexp[h] = ok ? a.exps[n * a.G + (ic >> 5)] : 0;
-      if (ok) {
-        if (a.vec_x) xcode[h] = *reinterpret_cast<const uint2*>(p);
-        else {
+      const int8_t* const q = p + (long)min(xr + (256 / XC) * h, last) * a.I;
+      if constexpr (VEC) xcode[set][h] = *reinterpret_cast<const uint2*>(q);
+      else {
+        uint2 w = {0, 0};
 #pragma unroll
-          for (int q = 0; q < 8; ++q)
-            if (q < in) (q < 4 ? xcode[h].x : xcode[h].y) |= (unsigned)(uint8_t)p[q] << (8 * (q & 3));
-        }
+        for (int j = 0; j < 8; ++j)
+          if (icv + j < a.I) (j < 4 ? w.x : w.y) |= (unsigned)(uint8_t)q[j] << (8 * (j & 3));
+        xcode[set][h] = w;
       }
     }
   };
-  auto load_y = [&](long n0) {   // P > 1, or rows that cannot be read 16 bytes at a time
-    if constexpr (P > 1) {
+  auto load_y = [&](long n0, int set) {
+    const int last = (int)min((long)KT, ne - n0) - 1;
+    const T* const p = static_cast<const T*>(a.dy) + n0 * a.O + ocv;
 #pragma unroll
-      for (int h = 0; h < YR; ++h) {
-        const long n = n0 + yr + (256 / YC) * h;
-        load8<T>(static_cast<const T*>(a.dy) + n * a.O + oc, n < ne ? on : 0, a.vec_dy, y[h]);
+    for (int h = 0; h < YR; ++h) {
+      const T* const q = p + (long)min(yr + (256 / YC) * h, last) * a.O;
+      if constexpr (VEC) y[set][h] = *reinterpret_cast<const t8*>(q);
+      else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) y[set][h][j] = ocv + j < a.O ? q[j] : (T)0.f;
       }
     }
   };
-  // brings dy's rows of a step (and, from registers, x's) into a stage
-  auto fill = [&](long n0, int stage, bool count) {
-    uint4* const to = smem + stage * kStage;
+  // bring a step's dy and x into a stage
+  auto fill_y = [&](long n0, int stage, bool count, int set) {
+    uint4* const to = own + stage * kStage;
+    const int rows = (int)min((long)KT, ne - n0);
     if constexpr (P == 1) {
-      if (a.vec_dy) {
+      if constexpr (VEC) {
 #pragma unroll
         for (int h = 0; h < NO; ++h)
           Fill<bf16_t, 128, KT>::issue(to + h * kY, static_cast<const bf16_t*>(a.dy) + n0 * a.O + o0 + 128 * h, a.O, a.O - o0 - 128 * h,
-                                       n0 + KT <= ne && o0 + 128 * h + 128 <= a.O, [&](int row) { return n0 + row < ne; });
+                                       n0 + KT <= ne && o0 + 128 * h + 128 <= a.O, [&](int row) { return n0 + row < ne; }, wave);
       } else {
 #pragma unroll
         for (int h = 0; h < YR; ++h) {
           const int row = yr + (256 / YC) * h;
-          float v[8];
-          load8<T>(static_cast<const T*>(a.dy) + (n0 + row) * a.O + oc, n0 + row < ne ? on : 0, false, v);
-          uint4 w;
-          unsigned* const wp = &w.x;
-#pragma unroll
-          for (int q = 0; q < 4; ++q) wp[q] = pair(__builtin_bit_cast(unsigned, v[2 * q]), __builtin_bit_cast(unsigned, v[2 * q + 1]));
-          to[(yc >> 4) * kY + Tl::at(row, yc & 15)] = w;
+          to[(yc >> 4) * kY + Tl::at(row, yc & 15)] = row < rows ? __builtin_bit_cast(uint4, y[set][h]) : uint4{0, 0, 0, 0};
         }
       }
     } else {
 #pragma unroll
       for (int h = 0; h < YR; ++h) {
+        const int row = yr + (256 / YC) * h;
+        float v[8];
+#pragma unroll
+        for (int q = 0; q < 8; ++q) v[q] = (float)y[set][h][q];
+        if (rows < KT) {
+#pragma unroll
+          for (int q = 0; q < 8; ++q) v[q] = row < rows ? v[q] : 0.f;
+        }
         if (count) {
 #pragma unroll
-          for (int q = 0; q < 8; ++q) db[q] += y[h][q];
+          for (int q = 0; q < 8; ++q) db[q] += v[q];
         }
-        const int at = (yc >> 4) * P * kY + Tl::at(yr + (256 / YC) * h, yc & 15);
+        const int at = (yc >> 4) * P * kY + Tl::at(row, yc & 15);
 #pragma unroll
         for (int p = 0; p < P; ++p) {
           uint4 w;
           unsigned* const wp = &w.x;
 #pragma unroll
           for (int q = 0; q < 4; ++q) {
-            float &lo = y[h][2 * q], &up = y[h][2 * q + 1];
+            float &lo = v[2 * q], &up = v[2 * q + 1];
             wp[q] = pair(__builtin_bit_cast(unsigned, lo), __builtin_bit_cast(unsigned, up));
             if (p + 1 < P) {   // exact: the bits below
               lo -= __builtin_bit_cast(float, hi_bits(lo));
@@ -301,27 +322,38 @@ __global__ __launch_bounds__(256, 2) void k_linear8_wgrad(WgradArgs a) {
         }
       }
     }
+  };
+  auto fill_x = [&](long n0, int stage, int set) {
+    uint4* const to = own + stage * kStage + P * NO * kY;
+    const int rows = (int)min((long)KT, ne - n0);
 #pragma unroll
-    for (int h = 0; h < XR; ++h) to[P * NO * kY + Tl::at(xr + 16 * h, xc)] = decode8(xcode[h], pow2_of(xexp[h]));
+    for (int h = 0; h < XR; ++h) {
+      const int row = xr + (256 / XC) * h;
+      to[(xc >> 4) * kY + Tl::at(row, xc & 15)] = decode8(xcode[set][h], pow2_of(row < rows ? xexp[set][h] : 0));
+    }
   };
   auto mine = [&](long n0) { return a.bias && (n0 - nb) / KT % a.ti == ji; };
   int stage = 0;
-  if (nb < ne) {
-    load_y(nb);
-    load_x(nb);
-    fill(nb, 0, mine(nb));
-    if (nb + KT < ne) { load_y(nb + KT); load_x(nb + KT); }
+  constexpr int STEP = 2 * KT;
+  constexpr bool kDirect = P == 1 && VEC;   // dy goes straight to LDS
+  auto load = [&](long n0, int set) {   // (behind the last step the last row again: no branch)
+    n0 = min(n0, ne - 1);
+    if constexpr (!kDirect) load_y(n0, set);
+    load_x(n0, set);
+  };
+  const long first = nb + half * KT;
+  if (first < ne) {
+    load(first, 0);
+    fill_y(first, 0, mine(first), 0);
+    fill_x(first, 0, 0);
+    load(first + STEP, 0);
+    if constexpr (!kDirect) load(first + 2 * STEP, 1);
   }
-  for (long n0 = nb; n0 < ne; n0 += KT) {
-    landed();
+  auto products = [&](long n0) {
     const unsigned cy = opaque(coly + stage * kStage * 16), cx = opaque(colx + stage * kStage * 16);
-    if (n0 + KT < ne) {
-      fill(n0 + KT, stage ^ 1, mine(n0 + KT));
-      if (n0 + 2 * KT < ne) { load_y(n0 + 2 * KT); load_x(n0 + 2 * KT); }
-    }
     if constexpr (P == 1) {
       if (mine(n0)) {
-        const uint4* const t = smem + stage * kStage + (yc >> 4) * kY;
+        const uint4* const t = own + stage * kStage + (yc >> 4) * kY;
 #pragma unroll
         for (int h = 0; h < YR; ++h) {
           const frag v = __builtin_bit_cast(frag, t[Tl::at(yr + (256 / YC) * h, yc & 15)]);
@@ -332,39 +364,94 @@ __global__ __launch_bounds__(256, 2) void k_linear8_wgrad(WgradArgs a) {
     }
 #pragma unroll
     for (int ks = 0; ks < KT / 16; ++ks) {
-      frag b[2];
+      frag b[NI];
 #pragma unroll
-      for (int n = 0; n < 2; ++n) b[n] = Tl::col(cx, 16 * ks, n);
+      for (int n = 0; n < NI; ++n) b[n] = Tl::col(cx, 16 * ks, n);
 #pragma unroll
       for (int p = P - 1; p >= 0; --p)   // small parts first
 #pragma unroll
         for (int m = 0; m < MO; ++m) {
           const frag f = Tl::col(cy, p * KT + 16 * ks, m);
 #pragma unroll
-          for (int n = 0; n < 2; ++n) acc[m][n] = Elem<bf16_t>::mma(f, b[n], acc[m][n]);
+          for (int n = 0; n < NI; ++n) acc[m][n] = Elem<bf16_t>::mma(f, b[n], acc[m][n]);
         }
     }
-    stage ^= 1;
-  }
-  float* const out = a.part + (long)split * a.O * a.I;
-#pragma unroll
-  for (int m = 0; m < MO; ++m)
-#pragma unroll
-    for (int n = 0; n < 2; ++n)
-#pragma unroll
-      for (int e = 0; e < 16; ++e) {
-        const int o = o0 + wo * 32 * MO + m * 32 + 8 * (e >> 2) + 4 * (lane >> 5) + (e & 3), i = i0 + wi * 64 + n * 32 + (lane & 31);
-        if (o < a.O && i < a.I) out[(long)o * a.I + i] = acc[m][n][e];
+  };
+  // The two halves share the SIMDs: where dy has to be split, one converts while the other one multiplies
+  auto step = [&](long n0, int set) {
+    if constexpr (kDirect) landed();
+    else __syncthreads();
+    const long now = n0 + half * KT, then = now + STEP;
+    const bool more = then < ne;
+    if constexpr (kDirect) {
+      if (more) {
+        fill_y(then, stage ^ 1, false, 0);
+        load(then + STEP, set ^ 1);
+        fill_x(then, stage ^ 1, set);
       }
-  if (a.bias) {
-    float* const lb = reinterpret_cast<float*>(smem);   // [256 / YC][8 * YC]
-    landed();
+      if (now < ne) products(now);
+    } else {
+      auto fill = [&] {
+        if (!more) return;
+        fill_y(then, stage ^ 1, mine(then), set);
+        fill_x(then, stage ^ 1, set);
+        load(then + 2 * STEP, set);
+      };
+      if (half == 0) fill();
+      if (now < ne) products(now);
+      if (half == 1) fill();
+    }
+    stage ^= 1;
+  };
+  for (long n0 = nb; n0 < ne; n0 += 2 * STEP) {
+    step(n0, 0);
+    if (n0 + STEP < ne) step(n0 + STEP, 1);
+  }
+  // each half gives the other one half of its accumulators and stores the sums of the rest
+  landed();
+  f32x4* const sums = reinterpret_cast<f32x4*>(smem) + wave * MO * NI * 4 * 64 + lane;
+  constexpr int MH = MO / 2;
+  auto give = [&](int m0) {
 #pragma unroll
-    for (int q = 0; q < 8; ++q) lb[yr * 8 * YC + 8 * yc + q] = db[q];
+    for (int m = 0; m < MH; ++m)
+#pragma unroll
+      for (int n = 0; n < NI; ++n)
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          const f32x16& v = acc[m0 + m][n];
+          sums[(((m0 + m) * NI + n) * 4 + q) * 64] = f32x4{v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]};
+        }
+  };
+  float* const out = a.part + (long)split * a.O * a.I;
+  auto store = [&](int m0) {
+#pragma unroll
+    for (int m = m0; m < m0 + MH; ++m)
+#pragma unroll
+      for (int n = 0; n < NI; ++n)
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          const f32x4 other = sums[((m * NI + n) * 4 + q) * 64];
+          const int o = o0 + wo * 32 * MO + m * 32 + 8 * q + 4 * (lane >> 5), i = i0 + wi * 32 * NI + n * 32 + (lane & 31);
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            if (o + e < a.O && i < a.I) out[(long)(o + e) * a.I + i] = acc[m][n][4 * q + e] + other[e];
+        }
+  };
+  if (half == 0) give(MH);
+  else give(0);
+  __syncthreads();
+  if (half == 0) store(0);
+  else store(MH);
+  if (a.bias) {
+    constexpr int NR = 512 / YC;
+    float* const lb = reinterpret_cast<float*>(smem);   // [NR][8 * YC]
+    __syncthreads();
+#pragma unroll
+    for (int q = 0; q < 8; ++q) lb[(half * (NR / 2) + yr) * 8 * YC + 8 * yc + q] = db[q];
     __syncthreads();
     if ((int)threadIdx.x < 8 * YC && o0 + (int)threadIdx.x < a.O) {
       float s = 0.f;
-      for (int r = 0; r < 256 / YC; ++r) s += lb[r * 8 * YC + threadIdx.x];
+      for (int r = 0; r < NR; ++r) s += lb[r * 8 * YC + threadIdx.x];
       a.part_b[((long)split * a.ti + ji) * a.O + o0 + threadIdx.x] = s;
     }
   }
@@ -450,21 +537,26 @@ template <typename T> struct KGelu { static auto get() { return k_pack8<T, true>
 template <typename T> struct KUnpack { static auto get() { return k_unpack8<T, false>; } };
 template <typename T> struct KGeluGrad { static auto get() { return k_unpack8<T, true>; } };
 
-// 256-channel tiles where they fit the output channels as well as 128-channel ones do.  Rows are split until two workgroups stand on every CU, each of
-// them with 256 rows at least: a shorter share costs more in partial tiles (8 bytes per element of dW and share) than it gains.
+// 256 channels where they fit as well as 128 do (bf16, 27552 rows, 512 x 2048: 284 us in 128 x 128 tiles, 102 in 256 x 128).  Rows are split until a workgroup
+// stands on every CU, each of them with 256 rows at least: a shorter share costs more in partial tiles (8 bytes per element of dW and share) than it gains.
 struct Cut8 { int wide, to, ti, splits; };
-Cut8 wgrad_cut(long N, int O, int I) {
+Cut8 wgrad_cut(int dtype, long N, int O, int I, bool vec) {
   Cut8 c;
-  c.wide = O > 128 && ((O + 127) / 128) % 2 == 0;
-  c.to = (O + (c.wide ? 255 : 127)) / (c.wide ? 256 : 128);
+  c.to = (O + 127) / 128;
   c.ti = (I + 127) / 128;
+  int& w = dtype == DT_BF16 ? c.to : c.ti;
+  c.wide = vec && w % 2 == 0;
+  if (c.wide) w /= 2;
   const long tiles = (long)c.to * c.ti;
-  long s = std::min<long>((512 + tiles - 1) / tiles, N / 256);
+  long s = std::min<long>((256 + tiles - 1) / tiles, N / 256);
   if (s > 8) s = s / 8 * 8;
   c.splits = (int)std::max<long>(1, std::min<long>(s, 64));
   return c;
 }
 size_t wgrad_floats(const Cut8& c, int O, int I) { return (size_t)c.splits * ((size_t)O * I + (size_t)c.ti * O); }
+size_t wgrad_bytes(int dtype, long N, int O, int I) {   // whatever the pointers turn out to be aligned to
+  return std::max(wgrad_floats(wgrad_cut(dtype, N, O, I, false), O, I), wgrad_floats(wgrad_cut(dtype, N, O, I, true), O, I)) * sizeof(float);
+}
 
 }  // namespace
 
@@ -528,7 +620,7 @@ extern "C" int fdx_linear8_weight_grad_workspace(int dtype, long long rows, int 
   if (!why) why = check(dtype, rows, in_features);
   if (!why && !bytes) why = "null size pointer";
   if (why) return fail(nullptr, FDX_E_ARG, "fdx_linear8_weight_grad_workspace: %s", why);
-  *bytes = wgrad_floats(wgrad_cut(rows, out_features, in_features), out_features, in_features) * sizeof(float);
+  *bytes = wgrad_bytes(dtype, rows, out_features, in_features);
   return FDX_OK;
 }
 
@@ -543,22 +635,23 @@ extern "C" int fdx_linear8_weight_grad(fdx_handle h, int dtype, const void* dy, 
   if (!why && (tiles > most / 64 || (long)out_features * in_features / 1024 + out_features / 32 + 2 > most)) why = "too many tiles for one launch";
   if (!why && (!dw || (rows > 0 && (!dy || !codes || !exps)))) why = "null tensor";
   if (why) return fail(h, FDX_E_ARG, "fdx_linear8_weight_grad: %s", why);
-  const Cut8 c = wgrad_cut(rows, out_features, in_features);
-  const size_t need = wgrad_floats(c, out_features, in_features) * sizeof(float);
+  const bool vec = aligned({dy}, out_features, 16) && aligned({codes}, in_features, 8);
+  const Cut8 c = wgrad_cut(dtype, rows, out_features, in_features, vec);
+  const size_t need = wgrad_bytes(dtype, rows, out_features, in_features);
   if (bytes < need || !workspace) return fail(h, FDX_E_ARG, "fdx_linear8_weight_grad: workspace of %zu bytes, %zu needed", bytes, need);
   WgradArgs a{};
   a.dy = dy; a.codes = codes; a.exps = exps; a.N = rows; a.O = out_features; a.I = in_features; a.G = (in_features + 31) / 32;
   a.to = c.to; a.ti = c.ti; a.splits = c.splits; a.bias = db != nullptr;
   a.rows = ((rows + a.splits - 1) / a.splits + 31) / 32 * 32;
-  a.vec_dy = aligned({dy}, a.O, 16); a.vec_x = aligned({codes}, a.I, 8);
   a.part = static_cast<float*>(workspace);
   a.part_b = a.part + (size_t)a.splits * a.O * a.I;
   DeviceScope dev(h->device);
   FDX_HIP(h, dev.err);
   hipStream_t s = as_stream(st);
-  const auto go = [&](auto narrow, auto wide) { return launch(c.wide ? wide : narrow, (unsigned)((long)c.to * c.ti * c.splits), 256, a, s); };
-  FDX_HIP(h, dtype == DT_F32 ? go(k_linear8_wgrad<float, 2>, k_linear8_wgrad<float, 4>) : dtype == DT_BF16 ? go(k_linear8_wgrad<bf16_t, 2>, k_linear8_wgrad<bf16_t, 4>)
-                                                                                              : go(k_linear8_wgrad<f16_t, 2>, k_linear8_wgrad<f16_t, 4>));
+  const auto go = [&](auto any, auto narrow, auto wide) { return launch(c.wide ? wide : vec ? narrow : any, (unsigned)((long)c.to * c.ti * c.splits), 512, a, s); };
+  FDX_HIP(h, dtype == DT_F32    ? go(k_linear8_wgrad<float, 2, 2, false>, k_linear8_wgrad<float, 2, 2, true>, k_linear8_wgrad<float, 2, 4, true>)
+             : dtype == DT_BF16 ? go(k_linear8_wgrad<bf16_t, 2, 2, false>, k_linear8_wgrad<bf16_t, 2, 2, true>, k_linear8_wgrad<bf16_t, 4, 2, true>)
+                                : go(k_linear8_wgrad<f16_t, 2, 2, false>, k_linear8_wgrad<f16_t, 2, 2, true>, k_linear8_wgrad<f16_t, 2, 4, true>));
   Join8Args j{a.part, a.part_b, dw, db, (long)a.O * a.I, a.splits, a.O, a.splits * a.ti, 0, 0};
   j.vec = j.n % 4 == 0 && (reinterpret_cast<uintptr_t>(dw) & 15) == 0 && (reinterpret_cast<uintptr_t>(workspace) & 15) == 0;
   j.main = (int)((j.n + 1023) / 1024);

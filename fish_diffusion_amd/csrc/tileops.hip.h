@@ -108,9 +108,9 @@ template <typename T, int DH, int TK> struct Fill {
   static constexpr int N = TK * Tl::CPR / 256, RPI = 64 / Tl::CPR;   // wave-instructions per wave, rows each covers
   static_assert(N * 256 == TK * Tl::CPR && 64 % Tl::CPR == 0, "whole rows per instruction");
   // rows t0 ... t0 + TK - 1 of `pitch` elements apart; `all`: every one of them exists and a row is DH elements (uniform), else has(row) says so, and chunks
-  // from D on are zeros
-  template <typename F> static __device__ inline void issue(uint4* lds, const T* t0, long pitch, int D, bool all, F&& has) {
-    const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), lane = threadIdx.x & 63;
+  // from D on are zeros; `part`: which of the four waves that share the tile this one is
+  template <typename F> static __device__ inline void issue(uint4* lds, const T* t0, long pitch, int D, bool all, F&& has, int part = (int)threadIdx.x >> 6) {
+    const int wave = __builtin_amdgcn_readfirstlane(part), lane = threadIdx.x & 63;
     const unsigned base = (unsigned)(size_t)(__attribute__((address_space(3))) uint4*)lds;
     if (all && pitch * TK * (long)sizeof(T) < (1L << 31)) {
       // one 32-bit lane offset (two where the swizzle alternates from instruction to instruction) on a scalar address: no vector arithmetic per step
