@@ -296,7 +296,8 @@ __global__ __launch_bounds__(256, (waves_of<T, DH>())) void k_attn_fwd(AttnArgs 
     for (int u = 0; u < NU; ++u)
 #pragma unroll
       for (int e = 0; e < 16; ++e) {
-        s[u][e] = exp2_(__builtin_fmaf(s[u][e], a.c, ref));
+        // fp32: the score is rounded as the reference was, so that the only key of a row has P = 1 exactly (16-bit results do not see the difference)
+        s[u][e] = exp2_(sizeof(T) == 4 ? s[u][e] * a.c + ref : __builtin_fmaf(s[u][e], a.c, ref));
         sum += s[u][e];
       }
     l += sum;
@@ -475,10 +476,12 @@ __global__ __launch_bounds__(256, (waves_of<T, DH>())) void k_attn_dq(AttnArgs a
     frag of[NS], go[NS];
     load_rows<T, DH>(go, static_cast<const T*>(a.go) + b * a.sgo.b + h * a.sgo.h + t * a.sgo.t, a.D, lane);
     load_rows<T, DH>(of, static_cast<const T*>(a.o) + b * a.so.b + h * a.so.h + t * a.so.t, a.D, lane);
+    // the diagonal of do o^T, by the instruction and in the order that dP is summed: a row of one key has o = v, dP - delta = 0 and gradients of exactly 0
+    f32x16 d = {0};
 #pragma unroll
-    for (int s = 0; s < NS; ++s)
+    for (int s = 0; s < NS; ++s) d = Elem<T>::mma(of[s], go[s], d);
 #pragma unroll
-      for (int j = 0; j < Elem<T>::VEC; ++j) delta = __builtin_fmaf((float)go[s][j], (float)of[s][j], delta);
+    for (int e = 0; e < 16; ++e) delta += 8 * (e >> 2) + 4 * hi + (e & 3) == (lane & 31) ? d[e] : 0.f;
     delta = half_sum(delta);
     if (empty) delta = 0.f;   // (whatever stands in do there)
     gf.set(go, own, wq, wk == 0, lane);

@@ -162,9 +162,11 @@ template <typename T, bool GRAD> __global__ __launch_bounds__(256) void k_unpack
 }
 
 // ---------------------------------------------------------------------------------------------------------------- weight gradient
-// A workgroup computes a tile of dW over its share of the rows n: 256 x 128 channels in two halves of four waves, each with all of the tile
-// ((32 MO) x (32 NI) a wave) over every other step of rows.  The halves' sums meet in LDS at the end, so a CU full of accumulators leaves one partial tile
-// instead of two (two independent workgroups of four waves: 59 + 14 us with the join against 55 + 8; fp32, 6888 rows, 2048 x 512).
+// A workgroup computes a tile of dW over its share of the rows n: 256 x 128 channels, (32 MO) x (32 NI) a wave.  fp32 and fp16: in two halves of four waves, each
+// with all of the tile over every other step of rows.  The halves' sums meet in LDS at the end, so a CU full of accumulators leaves one partial tile instead of
+// two, and one half splits dy while the other one multiplies (fp32, 6888 rows, 2048 x 512, with the join: 73 us in independent workgroups of four waves, 63 so).
+// bf16: independent workgroups of four waves, two on a CU; there is little to convert, and halves wait for each other (27552 rows, 512 x 2048, with pack and
+// join: 136 us, 144 in halves).
 // KT rows of dy (in bf16 planes) and of x8 (decoded) stand in LDS, two stages per half, both read as column fragments by transposing reads: MO + NI fragments
 // feed MO * NI matrix instructions.  bf16 dy goes straight to LDS, and the 256 are its channels: decoding x is all the arithmetic (per product least so).
 // The wider types pass registers to be split, the 256 are x's: splitting is the arithmetic then.
@@ -201,21 +203,22 @@ __device__ inline uint4 decode8(uint2 c, float scale) {
   return w;
 }
 
+template <typename T> constexpr int halves() { return Planes<T>::n == 1 ? 1 : 2; }
 template <typename T, int MO, int NI, bool VEC>
-__global__ __launch_bounds__(512, 2) void k_linear8_wgrad(WgradArgs a) {
+__global__ __launch_bounds__(256 * halves<T>(), 2) void k_linear8_wgrad(WgradArgs a) {
   typedef Tile<bf16_t, 128> Tl;
   typedef Elem<bf16_t>::frag frag;
-  constexpr int P = Planes<T>::n, KT = P == 1 ? 32 : 16, NO = MO / 2, NX = NI / 2;   // NO, NX: 128-channel tiles of dy and x
+  constexpr int P = Planes<T>::n, HV = halves<T>(), KT = P == 1 ? 32 : 16, NO = MO / 2, NX = NI / 2;   // NO, NX: 128-channel tiles of dy and x
   constexpr int kY = KT * 16, kStage = (P * NO + NX) * kY;   // in 16-byte units; kY: one tile
-  constexpr int kSum = 256 * MO * NI * 4;   // one half's accumulators
-  __shared__ __attribute__((aligned(1024))) uint4 smem[4 * kStage > kSum ? 4 * kStage : kSum];
+  constexpr int kSum = HV > 1 ? 256 * MO * NI * 4 : 0;   // one half's accumulators
+  __shared__ __attribute__((aligned(1024))) uint4 smem[2 * HV * kStage > kSum ? 2 * HV * kStage : kSum];
   const int per = a.to * a.ti;
   int split, j;
   if (a.splits % 8 == 0) { split = (blockIdx.x & 7) + 8 * ((blockIdx.x >> 3) / per); j = (blockIdx.x >> 3) % per; }
   else { split = blockIdx.x / per; j = blockIdx.x % per; }
   const int jo = j / a.ti, ji = j % a.ti, o0 = jo * 128 * NO, i0 = ji * 128 * NX;
   const int lane = threadIdx.x & 63, wave = (threadIdx.x >> 6) & 3, wo = wave >> 1, wi = wave & 1, tid = threadIdx.x & 255;
-  const int half = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 8);
+  const int half = HV > 1 ? __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 8) : 0;
   uint4* const own = smem + half * 2 * kStage;
   // staging of x: 8 columns of XR rows; of dy (through registers): 8 columns of YR rows
   constexpr int XC = 16 * NX, XR = KT * XC / 256, YC = 16 * NO, YR = KT * YC / 256;
@@ -334,7 +337,7 @@ __global__ __launch_bounds__(512, 2) void k_linear8_wgrad(WgradArgs a) {
   };
   auto mine = [&](long n0) { return a.bias && (n0 - nb) / KT % a.ti == ji; };
   int stage = 0;
-  constexpr int STEP = 2 * KT;
+  constexpr int STEP = HV * KT;
   constexpr bool kDirect = P == 1 && VEC;   // dy goes straight to LDS
   auto load = [&](long n0, int set) {   // (behind the last step the last row again: no branch)
     n0 = min(n0, ne - 1);
@@ -425,29 +428,32 @@ __global__ __launch_bounds__(512, 2) void k_linear8_wgrad(WgradArgs a) {
   float* const out = a.part + (long)split * a.O * a.I;
   auto store = [&](int m0) {
 #pragma unroll
-    for (int m = m0; m < m0 + MH; ++m)
+    for (int m = m0; m < m0 + MO / HV; ++m)
 #pragma unroll
       for (int n = 0; n < NI; ++n)
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
-          const f32x4 other = sums[((m * NI + n) * 4 + q) * 64];
+          f32x4 other = {0, 0, 0, 0};
+          if constexpr (HV > 1) other = sums[((m * NI + n) * 4 + q) * 64];
           const int o = o0 + wo * 32 * MO + m * 32 + 8 * q + 4 * (lane >> 5), i = i0 + wi * 32 * NI + n * 32 + (lane & 31);
 #pragma unroll
           for (int e = 0; e < 4; ++e)
             if (o + e < a.O && i < a.I) out[(long)(o + e) * a.I + i] = acc[m][n][4 * q + e] + other[e];
         }
   };
-  if (half == 0) give(MH);
-  else give(0);
-  __syncthreads();
-  if (half == 0) store(0);
-  else store(MH);
+  if constexpr (HV > 1) {
+    if (half == 0) give(MH);
+    else give(0);
+    __syncthreads();
+    if (half == 0) store(0);
+    else store(MH);
+  } else store(0);
   if (a.bias) {
-    constexpr int NR = 512 / YC;
+    constexpr int NR = 256 * HV / YC;
     float* const lb = reinterpret_cast<float*>(smem);   // [NR][8 * YC]
     __syncthreads();
 #pragma unroll
-    for (int q = 0; q < 8; ++q) lb[(half * (NR / 2) + yr) * 8 * YC + 8 * yc + q] = db[q];
+    for (int q = 0; q < 8; ++q) lb[(half * (256 / YC) + yr) * 8 * YC + 8 * yc + q] = db[q];
     __syncthreads();
     if ((int)threadIdx.x < 8 * YC && o0 + (int)threadIdx.x < a.O) {
       float s = 0.f;
@@ -537,8 +543,8 @@ template <typename T> struct KGelu { static auto get() { return k_pack8<T, true>
 template <typename T> struct KUnpack { static auto get() { return k_unpack8<T, false>; } };
 template <typename T> struct KGeluGrad { static auto get() { return k_unpack8<T, true>; } };
 
-// 256 channels where they fit as well as 128 do (bf16, 27552 rows, 512 x 2048: 284 us in 128 x 128 tiles, 102 in 256 x 128).  Rows are split until a workgroup
-// stands on every CU, each of them with 256 rows at least: a shorter share costs more in partial tiles (8 bytes per element of dW and share) than it gains.
+// 256 channels where they fit as well as 128 do (bf16, 27552 rows, 512 x 2048: 284 us in 128 x 128 tiles, 102 in 256 x 128).  Rows are split until eight
+// waves stand on every CU, each workgroup with 256 rows at least: a shorter share costs more in partial tiles (8 bytes per element of dW and share) than it gains.
 struct Cut8 { int wide, to, ti, splits; };
 Cut8 wgrad_cut(int dtype, long N, int O, int I, bool vec) {
   Cut8 c;
@@ -548,7 +554,8 @@ Cut8 wgrad_cut(int dtype, long N, int O, int I, bool vec) {
   c.wide = vec && w % 2 == 0;
   if (c.wide) w /= 2;
   const long tiles = (long)c.to * c.ti;
-  long s = std::min<long>((256 + tiles - 1) / tiles, N / 256);
+  const long want = dtype == DT_BF16 ? 512 : 256;
+  long s = std::min<long>((want + tiles - 1) / tiles, N / 256);
   if (s > 8) s = s / 8 * 8;
   c.splits = (int)std::max<long>(1, std::min<long>(s, 64));
   return c;
@@ -648,7 +655,7 @@ extern "C" int fdx_linear8_weight_grad(fdx_handle h, int dtype, const void* dy, 
   DeviceScope dev(h->device);
   FDX_HIP(h, dev.err);
   hipStream_t s = as_stream(st);
-  const auto go = [&](auto any, auto narrow, auto wide) { return launch(c.wide ? wide : vec ? narrow : any, (unsigned)((long)c.to * c.ti * c.splits), 512, a, s); };
+  const auto go = [&](auto any, auto narrow, auto wide) { return launch(c.wide ? wide : vec ? narrow : any, (unsigned)((long)c.to * c.ti * c.splits), dtype == DT_BF16 ? 256 : 512, a, s); };
   FDX_HIP(h, dtype == DT_F32    ? go(k_linear8_wgrad<float, 2, 2, false>, k_linear8_wgrad<float, 2, 2, true>, k_linear8_wgrad<float, 2, 4, true>)
              : dtype == DT_BF16 ? go(k_linear8_wgrad<bf16_t, 2, 2, false>, k_linear8_wgrad<bf16_t, 2, 2, true>, k_linear8_wgrad<bf16_t, 4, 2, true>)
                                 : go(k_linear8_wgrad<f16_t, 2, 2, false>, k_linear8_wgrad<f16_t, 2, 2, true>, k_linear8_wgrad<f16_t, 2, 4, true>));

@@ -339,3 +339,23 @@ def test_c_entries_refuse_strides_and_workspaces():
     torch.cuda.synchronize()
     want = torch.softmax((q[:, :1].double() @ k.double().transpose(-1, -2)), -1) @ v.double()
     assert (out.double() - want).abs().max() < 1e-3     # scores of up to 60 in sums of 32 products: 33 * 60 * 2^-24 = 1.2e-4 of P, |v| <= 4
+
+
+@pytest.mark.parametrize("t", list(T))
+@pytest.mark.parametrize("shape", [(2, 4, 2, 300, 1, 32), (1, 8, 8, 17, 1, 64), (2, 4, 4, 40, 700, 128), (16, 40, 40, 70, 5, 40)], ids=str)
+def test_rows_of_one_key(t, shape):
+    """One visible key: out is its value, dq and dk are exactly 0 (P = 1 whatever the score), dv the sum of grad_out."""
+    import fish_diffusion_amd as fda
+    q, k, v, do = inputs(T[t], *shape)
+    B, H, Hkv, Tq, Tk, D = shape
+    mask = torch.ones(B, Tk, dtype=torch.bool, device="cuda")
+    only = [(5 * b + 1) % Tk for b in range(B)]
+    for b, i in enumerate(only):
+        mask[b, i] = False
+    out, lse = fda.attention_forward(q, k, v, mask)
+    dq, dk, dv = fda.attention_backward(do, q, k, v, out, lse, mask)
+    at = torch.tensor(only, device="cuda")[:, None, None, None].expand(B, Hkv, 1, D)
+    assert torch.equal(out, v.gather(2, at).repeat_interleave(H // Hkv, 1).expand_as(out))
+    assert not dq.any() and not dk.any()
+    assert not dv.masked_fill(~mask[:, None, :, None], 0).any()
+    assert dv.any()
