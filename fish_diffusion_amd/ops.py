@@ -117,14 +117,15 @@ def _workspace_bytes(fn, *args) -> int:
     return n.value
 
 
-def _workspace(n: int, device):
-    return torch.empty(n, dtype=torch.uint8, device=device) if n else None
+def _workspace(n: int, like):
+    return like.new_empty((n,), dtype=torch.uint8) if n else None   # (new_empty: 1 us a call less than torch.empty with a device)
 
 
 # ------------------------------------------------------------------------------------------------------------- attention
 @functools.lru_cache(maxsize=1024)
 def _attn_plan(dtype, qs, ks, vs, causal, scale):
-    """What a call of these types and sizes needs (sizes only, no tensors): its C description, elements per 16 bytes, bytes of workspace each way."""
+    """What a call of these types and sizes needs (sizes only, no tensors): its C description, elements per 16 bytes, bytes of workspace each way, lse's
+    shape, and the strides of out / dq and of dk / dv -- [B, H, T, D] that lies in memory as [B, T, H, D]: joining the heads afterwards is a view."""
     if len(qs) != 4 or len(ks) != 4 or len(vs) != 4:
         raise ValueError("attention: q, k and v must be [batch, heads, length, channels] tensors")
     dt = _lib.DTYPES.get(dtype)
@@ -142,7 +143,8 @@ def _attn_plan(dtype, qs, ks, vs, causal, scale):
         raise ValueError(f"attention: scale must be positive and finite, got {scale}")
     desc = _lib.AttnDesc(dt, B, H, Hkv, Tq, Tk, D, int(causal), scale)
     lib = _lib.lib()
-    return desc, 4 if dt == 0 else 8, _workspace_bytes(lib.fdx_attn_forward_workspace, desc), _workspace_bytes(lib.fdx_attn_backward_workspace, desc)
+    return (desc, 4 if dt == 0 else 8, _workspace_bytes(lib.fdx_attn_forward_workspace, desc), _workspace_bytes(lib.fdx_attn_backward_workspace, desc),
+            (B, H, Tq), (Tq * H * D, D, H * D, 1), (Tk * Hkv * D, D, Hkv * D, 1))
 
 
 def _attn_check(q, k, v, key_mask, causal, scale):
@@ -166,11 +168,9 @@ def _attn_check(q, k, v, key_mask, causal, scale):
     return plan, key_mask
 
 
-def _new_rows(t: torch.Tensor):
-    """An uninitialised tensor of t's [B, H, T, D] shape that lies in memory as [B, T, H, D] -- joining the heads afterwards is a view -- and its description."""
-    B, H, T, D = t.shape
-    strides = (T * H * D, D, H * D, 1)
-    new = torch.empty_strided(t.shape, strides, dtype=t.dtype, device=t.device)
+def _new_rows(t: torch.Tensor, strides):
+    """An uninitialised tensor of t's shape and its description."""
+    new = t.new_empty_strided(t.shape, strides)
     return new, _lib.Bht(new.data_ptr() or None, *strides[:3])
 
 
@@ -181,12 +181,11 @@ def attention_forward(q, k, v, key_mask=None, causal=False, scale=None):
     key_mask [B, Tk], true = masked (whatever masked keys and values hold, NaN included, is never used); causal: query i sees keys up to
     i + Tk - Tq; scale defaults to D ** -0.5.  A row that sees no key is 0 (lse -inf).  Any strides; channels that are not contiguous or not
     16-byte aligned are copied first.  No autograd graph (`attention` builds one)."""
-    (desc, vec, n, _), key_mask = _attn_check(q, k, v, key_mask, causal, scale)
+    (desc, vec, n, _, lse_shape, rows, _), key_mask = _attn_check(q, k, v, key_mask, causal, scale)
     (q, aq), (k, ak), (v, av) = _arg(q, vec), _arg(k, vec), _arg(v, vec)
-    device = q.device
-    out, ao = _new_rows(q)
-    lse = torch.empty(q.shape[:3], dtype=torch.float32, device=device)
-    h, ws = _handle(device), _workspace(n, device)
+    out, ao = _new_rows(q, rows)
+    lse = q.new_empty(lse_shape, dtype=torch.float32)
+    h, ws = _handle(q.device), _workspace(n, q)
     with h.lock:
         rc = _lib.lib().fdx_attn_forward(h.h, desc, aq, ak, av, _p(key_mask), ao, lse.data_ptr(), _p(ws), n, _stream(h))
         if rc:
@@ -197,17 +196,17 @@ def attention_forward(q, k, v, key_mask=None, causal=False, scale=None):
 def attention_backward(grad_out, q, k, v, out, lse, key_mask=None, causal=False, scale=None):
     """(dq, dk, dv) of `attention_forward` called with the same arguments, from grad_out and its results.  dk / dv are summed over the query
     heads that share a key / value head; masked keys get 0, rows that see no key give 0 whatever grad_out holds there."""
-    (desc, vec, _, n), key_mask = _attn_check(q, k, v, key_mask, causal, scale)
+    (desc, vec, _, n, lse_shape, rows, keys), key_mask = _attn_check(q, k, v, key_mask, causal, scale)
     _same(q, "attention_backward", grad_out=grad_out, out=out)
     if grad_out.shape != q.shape or out.shape != q.shape:
         raise ValueError(f"attention_backward: grad_out {tuple(grad_out.shape)} and out {tuple(out.shape)} must have q's shape {tuple(q.shape)}")
     device = q.device
-    if lse.shape != q.shape[:3] or lse.dtype != torch.float32 or lse.device != device:
-        raise ValueError(f"attention_backward: lse must be the forward's float32 {tuple(q.shape[:3])} on {device}")
+    if lse.shape != lse_shape or lse.dtype != torch.float32 or lse.device != device:
+        raise ValueError(f"attention_backward: lse must be the forward's float32 {lse_shape} on {device}")
     (grad_out, ag), (q, aq), (k, ak), (v, av), (out, ao) = (_arg(t, vec) for t in (grad_out, q, k, v, out))
     lse = lse.contiguous()
-    (dq, adq), (dk, adk), (dv, adv) = _new_rows(q), _new_rows(k), _new_rows(v)
-    h, ws = _handle(device), _workspace(n, device)
+    (dq, adq), (dk, adk), (dv, adv) = _new_rows(q, rows), _new_rows(k, keys), _new_rows(v, keys)
+    h, ws = _handle(device), _workspace(n, q)
     with h.lock:
         rc = _lib.lib().fdx_attn_backward(h.h, desc, ag, aq, ak, av, ao, lse.data_ptr(), _p(key_mask), adq, adk, adv, _p(ws), n, _stream(h))
         if rc:
@@ -328,7 +327,7 @@ def residual_norm_forward(x, block, gate=None, residual_scale=1.0, post_norm=Non
     x, block, gate = _packed_rows(x), _packed_rows(block), _packed_rows(gate)
     h_out = torch.empty_like(x) if need_h else None
     y = torch.empty_like(x) if nw is not None else None
-    stats = torch.empty(x.shape[:-1] + (4,), dtype=torch.float32, device=x.device)
+    stats = x.new_empty((*x.shape[:-1], 4), dtype=torch.float32)
     if x.numel():
         h = _handle(x.device)
         with h.lock:
@@ -360,7 +359,7 @@ def residual_norm_backward(grad_h, grad_y, x, block, stats, gate=None, residual_
             if t is not None:
                 t.zero_()
     else:
-        h, ws = _handle(x.device), _workspace(n, x.device)
+        h, ws = _handle(x.device), _workspace(n, x)
         with h.lock:
             rc = _lib.lib().fdx_resnorm_backward(h.h, desc, *[_p(t) for t in (grad_h, grad_y, x, block, gate_c, pw, pb, nw, nb, stats, dx, dblock, dgate, *grads)],
                                                  _p(ws), n, _stream(h))
@@ -419,7 +418,7 @@ def _packed_ok(p: Packed8, what: str) -> Packed8:
 
 
 def _new_packed(x: torch.Tensor) -> Packed8:
-    return Packed8(torch.empty_like(x, dtype=torch.int8), torch.empty(x.shape[:-1] + ((x.shape[-1] + 31) // 32,), dtype=torch.uint8, device=x.device))
+    return Packed8(torch.empty_like(x, dtype=torch.int8), x.new_empty((*x.shape[:-1], (x.shape[-1] + 31) // 32), dtype=torch.uint8))
 
 
 def pack8(x) -> Packed8:
@@ -445,12 +444,17 @@ def unpack8(packed: Packed8, dtype=torch.float32) -> torch.Tensor:
     p = _packed_ok(packed, "unpack8")
     if dtype not in _lib.DTYPES:
         raise TypeError(f"unpack8: {dtype} is not one of float32, bfloat16, float16")
-    out = torch.empty(p.codes.shape, dtype=dtype, device=p.codes.device)
+    out = p.codes.new_empty(p.codes.shape, dtype=dtype)
     h = _handle(out.device)
     with h.lock:
         _lib.check(_lib.lib().fdx_unpack8(h.h, _lib.DTYPES[dtype], _p(p.codes), _p(p.exponents), *_rows_of(p.codes, "unpack8", "codes"), _p(out),
                                           _stream(h)), h.h)
     return out
+
+
+@functools.lru_cache(maxsize=1024)
+def _weight_grad_bytes(dt, N, O, I) -> int:
+    return _workspace_bytes(_lib.lib().fdx_linear8_weight_grad_workspace, dt, N, O, I)
 
 
 def linear8_weight_grad(dy, packed: Packed8, bias=True, dtype=None):
@@ -469,11 +473,11 @@ def linear8_weight_grad(dy, packed: Packed8, bias=True, dtype=None):
         raise ValueError(f"linear8_weight_grad: dy on {dy.device}, packed input on {p.codes.device}")
     I = p.codes.shape[-1]
     dy = _packed_rows(dy)
-    dw = torch.empty(O, I, dtype=dtype, device=dy.device)
-    db = torch.empty(O, dtype=dtype, device=dy.device) if bias else None
+    dw = dy.new_empty((O, I), dtype=dtype)
+    db = dy.new_empty((O,), dtype=dtype) if bias else None
     h, lib = _handle(dy.device), _lib.lib()
-    n = _workspace_bytes(lib.fdx_linear8_weight_grad_workspace, dt, N, O, I)
-    ws = _workspace(n, dy.device)
+    n = _weight_grad_bytes(dt, N, O, I)
+    ws = _workspace(n, dy)
     with h.lock:
         _lib.check(lib.fdx_linear8_weight_grad(h.h, dt, _p(dy), _p(p.codes), _p(p.exponents), N, O, I, _lib.DTYPES[dtype], _p(dw),
                                                _p(db), _p(ws), n, _stream(h)), h.h)
