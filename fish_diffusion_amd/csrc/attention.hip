@@ -35,7 +35,7 @@ struct AttnArgs {
 };
 
 // Two waves on a SIMD (256 registers each): the exponentials of one run under the matrix instructions of the other.  fp32 at head size 128 holds 128
-// accumulators and as many operands and stays at one.  (bf16, head size 128, 2 x 16 x 4096 causal forward: 353 us with one wave, 238 with two.)
+// accumulators and as many operands and stays at one.  (bf16, head size 128, 2 x 16 / 4 x 4096 causal: dq 540 us where one is asked for, 268 so; dk / dv 511, 352.)
 template <typename T, int DH> constexpr int waves_of() { return sizeof(T) == 4 && DH == 128 ? 1 : 2; }
 
 constexpr float kLn2 = 0.69314718055994530942f, kLog2e = 1.44269504088896340736f;
@@ -301,7 +301,7 @@ __global__ __launch_bounds__(256, (waves_of<T, DH>())) void k_attn_fwd(AttnArgs 
         sum += s[u][e];
       }
     l += sum;
-    __builtin_amdgcn_s_setprio(1);   // this wave's products before the other one's exponentials, which then run under them: 214 -> 209 us
+    __builtin_amdgcn_s_setprio(1);   // this wave's products before the other one's exponentials, which then run under them: 172 -> 168 us
 #pragma unroll
     for (int u = 0; u < NU; ++u)
 #pragma unroll
@@ -523,7 +523,7 @@ __global__ __launch_bounds__(256, (waves_of<T, DH>())) void k_attn_dq(AttnArgs a
 #pragma unroll
     for (int u = 0; u < NU; ++u) {
       f32x16 s = {0}, dp = {0};
-      __builtin_amdgcn_s_setprio(1);   // as in the forward, around the products with the longer chains: 377 -> 348 us
+      __builtin_amdgcn_s_setprio(1);   // as in the forward, around the products with the longer chains: 292 -> 268 us
 #pragma unroll
       for (int i = 0; i < NS; ++i) {
         s = Elem<T>::mma(Tl::row(row, 32 * u, i), qf[i], s);
@@ -821,7 +821,6 @@ __global__ __launch_bounds__(256, (waves_of<T, DH>())) void k_attn_dkv(AttnArgs 
         }
       }
       if constexpr (kScaled) rs.fit<MT>(s, dk);
-      __builtin_amdgcn_s_setprio(1);   // as in the forward: 373 -> 367 us
 #pragma unroll
       for (int i = 0; i < NP; ++i) {
         const frag pf = acc_frag<T>(p, i), df = acc_frag<T>(s, i);
@@ -831,7 +830,6 @@ __global__ __launch_bounds__(256, (waves_of<T, DH>())) void k_attn_dkv(AttnArgs 
           dk[m] = Elem<T>::mma(Tl::col(col, 32 * u + KS * i, m), df, dk[m]);
         }
       }
-      __builtin_amdgcn_s_setprio(0);
     }
   }
   float f = a.scale, fv = PShift<T>::back;

@@ -412,12 +412,24 @@ const char* check(const fdx_resnorm_desc* d) {
   return nullptr;
 }
 
-// Cut of the backward pass.  About a thousand workgroups fill the chip four times over; a gate row is never shared by two cuts of another one.
-// Gate rows shorter than 8 rows per unit are summed and written where they are read.
+// 8 channels a thread (16 above 4096 channels) and as many waves as that takes: the backward pass holds five sums and five values per channel, and with 8 of
+// them two waves fit on a SIMD.  (8 / 16 channels, backward, us: 16 x 861 x 512 fp32 30 / 55, 8 x 2048 x 2048 bf16 96 / 118.)
+struct Shape { int vec, it, nw; };
+Shape shape_of(const fdx_resnorm_desc* d, bool vec) {
+  const int v = !vec ? 1 : d->dtype == DT_F32 ? 4 : 8, C = d->channels;
+  return C <= 4096 ? Shape{v, 8 / v, C <= 512 ? 1 : C <= 1024 ? 2 : C <= 2048 ? 4 : 8} : Shape{v, 16 / v, 8};
+}
+int units_of(Shape sh) { return sh.nw == 1 ? 4 : 1; }   // rows a workgroup works on at a time
+
+// Cut of the backward pass: as many workgroups as the chip holds (two waves on a SIMD), one round of them; a unit has four rows at least.  More or fewer leave
+// places empty in the last round (256 / 384 / 512 / 768 / 1024 workgroups of four waves, us: 16 x 861 x 512 fp32 31.3 / 30.3 / 29.8 / 34.3 / 33.2,
+// 8 x 2048 x 2048 bf16 129 / 120 / 96 / 118 / 100).  A gate row is never shared by two cuts of another one.
+// Gate rows of which there are more than workgroups are summed and written where they are read.
 struct Cut { int wgs, cuts, flush; long groups, per; };
-Cut cut_of(const fdx_resnorm_desc* d, int units) {
+Cut cut_of(const fdx_resnorm_desc* d, Shape sh) {
   Cut c{};
-  const long N = d->rows, want = std::max<long>(1, std::min<long>(1024, (N + 4 * units - 1) / (4 * units)));
+  const int units = units_of(sh);
+  const long N = d->rows, room = 2048 / std::max(units, sh.nw), want = std::max<long>(1, std::min<long>(room, (N + 4 * units - 1) / (4 * units)));
   const bool many = d->gate_rows > 1 && d->gate_rows < N;
   c.groups = many ? N / d->gate_rows : 1;
   c.per = many ? d->gate_rows : N;
@@ -428,14 +440,6 @@ Cut cut_of(const fdx_resnorm_desc* d, int units) {
     c.wgs = (int)c.groups * c.cuts;
   }
   return c;
-}
-
-// 8 channels a thread (16 above 4096 channels) and as many waves as that takes: the backward pass holds five sums and five values per channel, and with 8 of
-// them two to three workgroups of four waves fit on a CU.
-struct Shape { int vec, it, nw; };
-Shape shape_of(const fdx_resnorm_desc* d, bool vec) {
-  const int v = !vec ? 1 : d->dtype == DT_F32 ? 4 : 8, C = d->channels;
-  return C <= 4096 ? Shape{v, 8 / v, C <= 512 ? 1 : C <= 1024 ? 2 : C <= 2048 ? 4 : 8} : Shape{v, 16 / v, 8};
 }
 
 template <typename T, int VEC, bool BWD, int IT, int NW> hipError_t run(const NormArgs& a, unsigned grid, hipStream_t s) {
@@ -456,7 +460,6 @@ template <bool BWD> hipError_t by_type(const fdx_resnorm_desc* d, const NormArgs
   if (d->dtype == DT_BF16) return one ? run<bf16_t, 1, BWD>(a, sh, grid, s) : run<bf16_t, 8, BWD>(a, sh, grid, s);
   return one ? run<f16_t, 1, BWD>(a, sh, grid, s) : run<f16_t, 8, BWD>(a, sh, grid, s);
 }
-int units_of(Shape sh) { return sh.nw == 1 ? 4 : 1; }
 
 NormArgs args_of(const fdx_resnorm_desc* d) {
   NormArgs a{};
@@ -495,7 +498,7 @@ extern "C" int fdx_resnorm_forward(fdx_handle h, const fdx_resnorm_desc* d, cons
 extern "C" int fdx_resnorm_backward_workspace(const fdx_resnorm_desc* d, size_t* bytes) {
   if (const char* why = check(d)) return fail(nullptr, FDX_E_ARG, "fdx_resnorm_backward_workspace: %s", why);
   if (!bytes) return fail(nullptr, FDX_E_ARG, "fdx_resnorm_backward_workspace: null size pointer");
-  *bytes = (size_t)cut_of(d, units_of(shape_of(d, true))).wgs * 5 * d->channels * sizeof(float);
+  *bytes = (size_t)cut_of(d, shape_of(d, true)).wgs * 5 * d->channels * sizeof(float);
   return FDX_OK;
 }
 
@@ -518,7 +521,7 @@ extern "C" int fdx_resnorm_backward(fdx_handle h, const fdx_resnorm_desc* d, con
   if (a.same_dx && (post_w || gate || d->residual_scale != 1.f))
     return fail(h, FDX_E_ARG, "fdx_resnorm_backward: dblock may be dx only where they are equal (no gate, no post norm, residual_scale 1)");
   const Shape sh = shape_of(d, vec_ok(d, {x, block, gate, post_w, post_b, pre_w, pre_b, grad_h, grad_y, dx, dblock, dgate}));
-  const Cut c = cut_of(d, units_of(sh));
+  const Cut c = cut_of(d, sh);
   const size_t need = (size_t)c.wgs * 5 * d->channels * sizeof(float);
   if (bytes < need || !workspace || (reinterpret_cast<uintptr_t>(workspace) & 15))
     return fail(h, FDX_E_ARG, "fdx_resnorm_backward: workspace of %zu bytes, %zu needed (16-byte aligned)", bytes, need);
