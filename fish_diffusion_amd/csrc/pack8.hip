@@ -49,8 +49,17 @@ struct EltArgs {
   int8_t* codes;
   uint8_t* exps;
   long N;
-  int C, G, vec, out_dt;
+  int C, G, vec;
 };
+// thread i of a pass: its first element, how many of its 8 exist, its group.  Whole groups in a row follow each other without gaps; otherwise the row is
+// found by a division (64 bits: as many instructions as a GELU of 4 elements).
+struct Eighth { long o, group; int n; };
+__device__ inline Eighth eighth(const EltArgs& a, long i) {
+  if (a.C % 32 == 0) return {8 * i, i >> 2, 8};
+  const long per = 4L * a.G, row = i / per;
+  const int q = (int)(i - row * per);
+  return {row * a.C + 8 * q, row * a.G + (q >> 2), a.C - 8 * q};
+}
 
 template <typename T> __device__ inline void load8(const T* p, int n, bool vec, float* v) {   // n of 8 valid
   if (vec && n >= 8) {
@@ -90,12 +99,10 @@ __device__ inline void load_codes(const int8_t* p, int n, bool vec, float scale,
 
 // codes of x; GELU: y = gelu(x) beside them
 template <typename T, bool GELU> __global__ __launch_bounds__(256) void k_pack8(EltArgs a) {
-  const long per = 4L * a.G, total = a.N * per;
+  const long total = a.N * 4L * a.G;
   const long first = (long)blockIdx.x * 256 + threadIdx.x, stride = (long)gridDim.x * 256;
   for (long i = first; i < total; i += stride) {   // (the four lanes of a group leave together: total and stride are multiples of 4)
-    const long row = i / per;
-    const int q = (int)(i - row * per), c = q * 8, n = a.C - c;
-    const long o = row * a.C + c;
+    const auto [o, group, n] = eighth(a, i);
     float v[8];
     load8<T>(static_cast<const T*>(a.x) + o, n, a.vec, v);
     unsigned top = 0;
@@ -120,7 +127,7 @@ template <typename T, bool GELU> __global__ __launch_bounds__(256) void k_pack8(
         for (int j = 0; j < 8; ++j)
           if (j < n) a.codes[o + j] = (int8_t)code[j];
       }
-      if ((q & 3) == 0) a.exps[row * a.G + (q >> 2)] = (uint8_t)e;
+      if ((i & 3) == 0) a.exps[group] = (uint8_t)e;
       if constexpr (GELU) {
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
@@ -136,14 +143,12 @@ template <typename T, bool GELU> __global__ __launch_bounds__(256) void k_pack8(
 
 // y = what the codes stand for; GRAD: y = dy * gelu'(that)
 template <typename T, bool GRAD> __global__ __launch_bounds__(256) void k_unpack8(EltArgs a) {
-  const long per = 4L * a.G, total = a.N * per;
+  const long total = a.N * 4L * a.G;
   for (long i = (long)blockIdx.x * 256 + threadIdx.x; i < total; i += (long)gridDim.x * 256) {
-    const long row = i / per;
-    const int q = (int)(i - row * per), c = q * 8, n = a.C - c;
+    const auto [o, group, n] = eighth(a, i);
     if (n <= 0) continue;
-    const long o = row * a.C + c;
     float v[8];
-    load_codes(a.codes + o, n, a.vec, pow2_of(a.exps[row * a.G + (q >> 2)]), v);
+    load_codes(a.codes + o, n, a.vec, pow2_of(a.exps[group]), v);
     if constexpr (GRAD) {
       float d[8];
       load8<T>(static_cast<const T*>(a.dy) + o, n, a.vec, d);
