@@ -821,6 +821,8 @@ __global__ __launch_bounds__(256, (waves_of<T, DH>())) void k_attn_dkv(AttnArgs 
         }
       }
       if constexpr (kScaled) rs.fit<MT>(s, dk);
+      // as in the forward; here it also keeps the compiler from moving the next rows' products in between, whose operands then spill (742 -> 933 us both ways)
+      __builtin_amdgcn_s_setprio(1);
 #pragma unroll
       for (int i = 0; i < NP; ++i) {
         const frag pf = acc_frag<T>(p, i), df = acc_frag<T>(s, i);
@@ -830,6 +832,7 @@ __global__ __launch_bounds__(256, (waves_of<T, DH>())) void k_attn_dkv(AttnArgs 
           dk[m] = Elem<T>::mma(Tl::col(col, 32 * u + KS * i, m), df, dk[m]);
         }
       }
+      __builtin_amdgcn_s_setprio(0);
     }
   }
   float f = a.scale, fv = PShift<T>::back;
