@@ -414,6 +414,8 @@ const char* check(const fdx_resnorm_desc* d) {
 
 // 8 channels a thread (16 above 4096 channels) and as many waves as that takes: the backward pass holds five sums and five values per channel, and with 8 of
 // them two waves fit on a SIMD.  (8 / 16 channels, backward, us: 16 x 861 x 512 fp32 30 / 55, 8 x 2048 x 2048 bf16 96 / 118.)
+// Above 4096 channels the backward pass spills (1024 x 8192: fp32 134 us, bf16 53; reading the parameters again for every row and loading no row ahead does not
+// save enough registers: 155, 56).
 struct Shape { int vec, it, nw; };
 Shape shape_of(const fdx_resnorm_desc* d, bool vec) {
   const int v = !vec ? 1 : d->dtype == DT_F32 ? 4 : 8, C = d->channels;
