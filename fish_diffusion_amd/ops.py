@@ -197,16 +197,17 @@ def attention_backward(grad_out, q, k, v, out, lse, key_mask=None, causal=False,
     """(dq, dk, dv) of `attention_forward` called with the same arguments, from grad_out and its results.  dk / dv are summed over the query
     heads that share a key / value head; masked keys get 0, rows that see no key give 0 whatever grad_out holds there."""
     (desc, vec, _, n, lse_shape, rows, keys), key_mask = _attn_check(q, k, v, key_mask, causal, scale)
-    _same(q, "attention_backward", grad_out=grad_out, out=out)
+    dev, dtype = q.get_device(), q.dtype
+    if grad_out.get_device() != dev or out.get_device() != dev or grad_out.dtype is not dtype or out.dtype is not dtype:
+        _same(q, "attention_backward", grad_out=grad_out, out=out)
     if grad_out.shape != q.shape or out.shape != q.shape:
         raise ValueError(f"attention_backward: grad_out {tuple(grad_out.shape)} and out {tuple(out.shape)} must have q's shape {tuple(q.shape)}")
-    device = q.device
-    if lse.shape != lse_shape or lse.dtype != torch.float32 or lse.device != device:
-        raise ValueError(f"attention_backward: lse must be the forward's float32 {lse_shape} on {device}")
+    if lse.shape != lse_shape or lse.dtype is not torch.float32 or lse.get_device() != dev:
+        raise ValueError(f"attention_backward: lse must be the forward's float32 {lse_shape} on {q.device}")
     (grad_out, ag), (q, aq), (k, ak), (v, av), (out, ao) = (_arg(t, vec) for t in (grad_out, q, k, v, out))
     lse = lse.contiguous()
     (dq, adq), (dk, adk), (dv, adv) = _new_rows(q, rows), _new_rows(k, keys), _new_rows(v, keys)
-    h, ws = _handle(device), _workspace(n, q)
+    h, ws = _handle(q.device), _workspace(n, q)
     with h.lock:
         rc = _lib.lib().fdx_attn_backward(h.h, desc, ag, aq, ak, av, ao, lse.data_ptr(), _p(key_mask), adq, adk, adv, _p(ws), n, _stream(h))
         if rc:
@@ -252,13 +253,13 @@ _NO_NORM = (None, None)
 
 def _packed_rows(t: Optional[torch.Tensor]) -> Optional[torch.Tensor]:
     """Contiguous and 16-byte aligned (a copy where it is not)."""
-    if t is None or t.numel() == 0:
+    if t is None or (t.is_contiguous() and not t.data_ptr() & 15):
         return t
-    return t if t.is_contiguous() and not t.data_ptr() & 15 else _copy(t)
+    return _copy(t)
 
 
 @functools.lru_cache(maxsize=1024)
-def _norm_plan(dtype, shape, param_dtypes, param_shapes, gate_dtype, gate_shape, residual_scale, kind, eps):
+def _norm_plan(dtype, shape, params, gate_dtype, gate_shape, residual_scale, kind, eps):   # params: (type, shape) or None each
     """The C description of a call of these types and sizes, and its backward pass's bytes of workspace."""
     dt = _lib.DTYPES.get(dtype)
     if dt is None:
@@ -270,12 +271,12 @@ def _norm_plan(dtype, shape, param_dtypes, param_shapes, gate_dtype, gate_shape,
         raise ValueError(f"residual_norm: kind must be 'layer' or 'rms', got {kind!r}")
     if not (math.isfinite(residual_scale) and eps >= 0.0 and math.isfinite(eps)):
         raise ValueError("residual_norm: residual_scale must be finite and eps finite and not negative")
-    pdt = set(t for t in param_dtypes if t is not None) or {dtype}
+    pdt = set(p[0] for p in params if p is not None) or {dtype}
     if len(pdt) > 1 or not pdt <= {dtype, torch.float32}:
         raise ValueError(f"residual_norm: the norms' weights and biases must all be {dtype} or all float32, got {sorted(map(str, pdt))}")
-    for sh in param_shapes:
-        if sh is not None and sh != (C_,):
-            raise ValueError(f"residual_norm: a norm's weight / bias has shape {tuple(sh)}, expected {(C_,)}")
+    for p in params:
+        if p is not None and p[1] != (C_,):
+            raise ValueError(f"residual_norm: a norm's weight / bias has shape {tuple(p[1])}, expected {(C_,)}")
     rows = 0
     if gate_shape is not None:
         if gate_dtype not in (dtype, torch.float32):
@@ -301,14 +302,13 @@ def _norm_args(x, block, gate, residual_scale, post_norm, pre_norm, kind, eps):
     if (post_norm and pw is None) or (pre_norm and nw is None):
         raise ValueError("residual_norm: post_norm and pre_norm must be None or (weight, bias or None)")
     params = (pw, pb, nw, nb)
-    plan = _norm_plan(x.dtype, x.shape, tuple([p if p is None else p.dtype for p in params]), tuple([p if p is None else p.shape for p in params]),
-                      None if gate is None else gate.dtype, None if gate is None else gate.shape, float(residual_scale), kind, float(eps))
+    plan = _norm_plan(x.dtype, x.shape, tuple([p if p is None else (p.dtype, p.shape) for p in params]), None if gate is None else gate.dtype,
+                      None if gate is None else gate.shape, float(residual_scale), kind, float(eps))
     if block.dtype is not x.dtype:
         raise ValueError(f"residual_norm: block is {block.dtype}, x {x.dtype}")
     dev = x.get_device()
-    for t in (block, gate, *params):
-        if t is not None and t.get_device() != dev:
-            raise ValueError(f"residual_norm: tensors on {t.device} and {x.device}")
+    if [True for t in (block, gate, *params) if t is not None and t.get_device() != dev]:
+        raise ValueError("residual_norm: tensors on different devices")
     if dev < 0:
         _lib.require_gpu(x, "residual_norm x")
     return plan, [p if p is None else _packed_rows(p) for p in params]
@@ -343,7 +343,7 @@ def residual_norm_backward(grad_h, grad_y, x, block, stats, gate=None, residual_
     residual_scale is 1, dx and dblock are equal and are ONE tensor.  The gate's gradient has the gate's shape."""
     (desc, n), (pw, pb, nw, nb) = _norm_args(x, block, gate, residual_scale, post_norm, pre_norm, kind, eps)
     for name, g in (("grad_h", grad_h), ("grad_y", grad_y)):
-        if g is not None and (g.shape != x.shape or g.dtype != x.dtype or g.device != x.device):
+        if g is not None and (g.shape != x.shape or g.dtype is not x.dtype or g.get_device() != x.get_device()):
             raise ValueError(f"residual_norm_backward: {name} must be {x.dtype} {tuple(x.shape)} on {x.device}")
     if grad_y is not None and nw is None:
         raise ValueError("residual_norm_backward: grad_y without a pre_norm")
