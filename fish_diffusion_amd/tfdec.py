@@ -108,7 +108,11 @@ class TransformerDecoderDenoiser(HipDenoiser):
         masks [B, T] with true = padding; gradients for the parameters and for x and conditioner where they ask for them.  It runs in the parameters'
         type (fp32, or bf16 / fp16 after `.to()`) on the parameters themselves: nothing is packed.  keep8=True keeps the inputs of the linear layers and
         GELUs in 8 bits instead of the parameters' type (`ops.pack8`): the result is as exact (GELU is evaluated by `ops.gelu8`), weight gradients and GELU's
-        derivative see inputs rounded to a step of at most 2/127 of the largest of their 32 neighbours."""
+        derivative see inputs rounded to a step of at most 2/127 of the largest of their 32 neighbours.  Autocast is not applied: the parameters' type rules."""
+        with torch.autocast(x.device.type, enabled=False):
+            return self._training_forward(x, diffusion_step, conditioner, x_masks, cond_masks, keep8)
+
+    def _training_forward(self, x, diffusion_step, conditioner, x_masks, cond_masks, keep8):
         assert x.dim() == 3, f"mel must be 3 dim tensor, but got {x.dim()}"
         sd = dict(self.named_parameters())
         w = sd["input_projection.0.weight"]

@@ -150,3 +150,17 @@ def test_capture_beside_a_live_graph_is_refused():
     with torch.cuda.graph(g):
         with pytest.raises(RuntimeError, match="outside this capture"):
             net.training_forward(x, step, cond)
+
+
+@pytest.mark.parametrize("keep8", [False, True])
+def test_autocast_is_not_applied(keep8):
+    net, _, x, step, cond, xm, cm, gy = setup()
+    x, step, cond, xm, cm, gy = (t.cuda() for t in (x, step, cond, xm, cm, gy))
+    got = []
+    for on in (False, True):
+        net.zero_grad()
+        with torch.autocast("cuda", dtype=torch.bfloat16, enabled=on):
+            y = net.training_forward(x, step, cond, xm, cm, keep8=keep8)
+        y.backward(gy)
+        got.append([y.detach()] + [p.grad.clone() for p in net.parameters()])
+    assert all(a.dtype == torch.float32 and torch.equal(a, b) for a, b in zip(*got))
