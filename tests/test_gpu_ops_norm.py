@@ -255,3 +255,30 @@ def test_only_the_normalised_result():
     assert torch.equal(lx.grad, fda.residual_norm_backward(None, gy, x, block, stats, **kw).dx)
     with pytest.raises(ValueError):
         fda.residual_norm(x, block, need_h=False)
+
+
+def test_one_tensor_as_both_inputs():
+    """x and block may be one tensor: their gradients, which are one tensor too where they are equal, add up."""
+    import fish_diffusion_amd as fda
+    g = torch.Generator(device="cuda").manual_seed(3)
+    x = torch.randn(5, 7, 64, generator=g, device="cuda")
+    w, gh, gy = (torch.randn(*s, generator=g, device="cuda") for s in ((64,), (5, 7, 64), (5, 7, 64)))
+    for leaf in (True, False):
+        t = x.clone().requires_grad_()
+        u = t if leaf else t * 1.0
+        h, y = fda.residual_norm(u, u, pre_norm=(w, None))
+        got, = torch.autograd.grad((h, y), t, (gh, gy))
+        t.grad = None
+        h, y = fda.residual_norm(u if leaf else t * 1.0, u if leaf else t * 1.0, pre_norm=(w, None))
+        torch.autograd.backward((h, y), (gh, gy))
+        d = x.double().requires_grad_()
+        z = 2 * d
+        ref = torch.nn.functional.layer_norm(z, (64,), w.double())
+        want, = torch.autograd.grad((z, ref), d, (gh.double(), gy.double()))
+        # 64 products a sum, |grad| and |normalised| up to 4 each, three such terms, doubled: 2 * 3 * 66 * 16 * 2^-24
+        assert (got.double() - want).abs().max() <= 4e-4 and torch.equal(t.grad, got)
+    a, b = x.clone().requires_grad_(), x.clone().requires_grad_()
+    h, y = fda.residual_norm(a, b, pre_norm=(w, None))
+    torch.autograd.backward((h, y), (gh, gy))
+    a.grad.zero_()                                       # (two parameters' gradients are two tensors)
+    assert b.grad.any()
